@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from .csrc import build as _build
+from .microscale import BLOCK, Matrix4, Rows8, matrix4  # noqa: F401  (part of this module's face)
 
 F32, BF16, F16 = 0, 1, 2
 _DTYPE_TAG = {torch.float32: F32, torch.bfloat16: BF16}
@@ -1770,6 +1771,112 @@ def linear(a: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
                            ctypes.byref(filed), _stream()))
     if kv is not None and filed.value:
         kv.done = True
+    return out
+
+
+# --------------------------------------- rows in 8 bits, weights in 4 bits --
+
+def _here(name: str, *tensors: torch.Tensor | None) -> None:
+    """Kernels run on the current device's current stream: tensors of another device are refused."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{name}: a tensor on {t.device}, the current device is cuda:{device}")
+
+
+def _stride(t: torch.Tensor) -> int:
+    """Numbers from a row to the next; of a single row, whose stride says nothing, its width."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rows8(x: torch.Tensor) -> Rows8:
+    """Rows [T, K] of float32 or bfloat16 (columns side by side; they may be columns of a wider matrix) in 8 bits: e4m3 numbers
+    with a power of two for every 32 columns (``microscale``)."""
+    lib = _ready()
+    if x.dim() != 2 or x.shape[1] < BLOCK or x.shape[1] % BLOCK or x.stride(1) != 1:
+        raise KernelError(f"rows8: rows must be [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(x.shape)}")
+    tag = _tag(x.dtype)
+    _here("rows8", x)
+    T, K = x.shape
+    out = Rows8.empty(T, K, x.device)
+    if T:
+        _launch(lib.ayk_rows8(_ptr(out.codes), _ptr(out.scales), ctypes.c_longlong(out.scales.stride(0)), _ptr(x),
+                              ctypes.c_longlong(_stride(x)), ctypes.c_longlong(T), ctypes.c_int(K), ctypes.c_int(tag), _stream()))
+    return out
+
+
+def rmsnorm_rows8(x: torch.Tensor, weight: torch.Tensor, eps: float, y: torch.Tensor | None = None) -> Rows8:
+    """x += y, in place on the float32 residual stream [T, K], and x / sqrt(mean(x^2) + eps) * weight of the new x in 8 bits.
+    ``y``: a sublayer's result, float32 or bfloat16 (None: x stays as it is).  x and y may be columns of wider matrices, but
+    not overlap."""
+    lib = _ready()
+    if x.dim() != 2 or x.dtype != torch.float32 or x.shape[1] < BLOCK or x.shape[1] % BLOCK or x.stride(1) != 1:
+        raise KernelError(f"rmsnorm_rows8: the stream must be float32 [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(x.shape)} of {x.dtype}")
+    T, K = x.shape
+    if y is not None and (T > 1 and x.stride(0) < K):
+        raise KernelError("rmsnorm_rows8: rows that are written must not overlap")
+    if _f32(weight, "weight").numel() != K:
+        raise KernelError("rmsnorm_rows8: weight must be float32 of the row width")
+    if y is not None and (y.shape != x.shape or y.stride(1) != 1):
+        raise KernelError("rmsnorm_rows8: y must have the stream's shape and unit column stride")
+    tag = F32 if y is None else _tag(y.dtype)
+    _here("rmsnorm_rows8", x, weight, y)
+    out = Rows8.empty(T, K, x.device)
+    if T:
+        _launch(lib.ayk_rmsnorm_rows8(_ptr(out.codes), _ptr(out.scales), ctypes.c_longlong(out.scales.stride(0)), _ptr(x),
+                                      ctypes.c_longlong(_stride(x)), _ptr(y), ctypes.c_longlong(0 if y is None else _stride(y)),
+                                      ctypes.c_int(tag), _ptr(weight), ctypes.c_longlong(T), ctypes.c_int(K), ctypes.c_float(eps), _stream()))
+    return out
+
+
+def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: str = "none", residual: torch.Tensor | None = None,
+            out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """act(a @ w^T + bias) (+ residual): rows in 8 bits times a weight in 4, products exact, sums, activation (as ``linear``) and
+    residual (float32; it may be ``out``) in 32-bit."""
+    lib = _ready()
+    T, K = a.codes.shape
+    N = w.shape[0]
+    if w.shape[1] != K:
+        raise KernelError(f"linear4: operands do not fit: rows {(T, K)}, weight {w.shape}")
+    if activation not in ACTIVATIONS:
+        raise KernelError(f"linear4: unknown activation {activation!r}; known: {sorted(ACTIVATIONS)}")
+    tag = _tag(out_dtype)
+    if out is not None and (tuple(out.shape) != (T, N) or out.dtype != out_dtype or not out.is_contiguous()):
+        raise KernelError("linear4: out must be a contiguous [T, N] tensor of the output dtype")
+    if bias is not None and _f32(bias, "bias").numel() != N:
+        raise KernelError("linear4: one bias per column")
+    if residual is not None and tuple(_f32(residual, "residual").shape) != (T, N):
+        raise KernelError("linear4: residual must have the output's shape")
+    _here("linear4", a.codes, w.codes, bias, residual, out)
+    if out is None:
+        out = torch.empty((T, N), dtype=out_dtype, device=a.codes.device)
+    if T:
+        _launch(lib.ayk_linear4(_ptr(out), _ptr(a.codes), ctypes.c_longlong(_stride(a.codes)), _ptr(a.scales),
+                                ctypes.c_longlong(_stride(a.scales)), _ptr(w.codes), _ptr(w.scales), _ptr(bias), _ptr(residual),
+                                ctypes.c_longlong(T), ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(ACTIVATIONS[activation]),
+                                ctypes.c_int(tag), _stream()))
+    return out
+
+
+def gated_linear4(a: Rows8, gate: Matrix4, up: Matrix4, activation: str = "silu") -> Rows8:
+    """act(a @ gate^T) * (a @ up^T) in 8 bits: the first half of a gated feed-forward, whose rows the second half's ``linear4``
+    reads.  Both products' sums, the activation and their product are 32-bit; the code is the one rounding."""
+    lib = _ready()
+    T, K = a.codes.shape
+    N = gate.shape[0]
+    if gate.shape != up.shape or gate.shape[1] != K:
+        raise KernelError(f"gated_linear4: operands do not fit: rows {(T, K)}, weights {gate.shape} and {up.shape}")
+    if N % BLOCK:
+        raise KernelError(f"gated_linear4: a row of {N} is not whole blocks of {BLOCK}")
+    if activation not in ACTIVATIONS:
+        raise KernelError(f"gated_linear4: unknown activation {activation!r}; known: {sorted(ACTIVATIONS)}")
+    _here("gated_linear4", a.codes, gate.codes, up.codes)
+    out = Rows8.empty(T, N, a.codes.device)
+    if T:
+        _launch(lib.ayk_gated_linear4(_ptr(out.codes), _ptr(out.scales), ctypes.c_longlong(out.scales.stride(0)), _ptr(a.codes),
+                                      ctypes.c_longlong(_stride(a.codes)), _ptr(a.scales), ctypes.c_longlong(_stride(a.scales)),
+                                      _ptr(gate.codes), _ptr(gate.scales), _ptr(up.codes), _ptr(up.scales), ctypes.c_longlong(T),
+                                      ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(ACTIVATIONS[activation]), _stream()))
     return out
 
 

@@ -1,0 +1,169 @@
+"""Rows in 8 bits and weights in 4 bits: formats, layouts and refusals, without a GPU."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from ayaka_py_b200 import ops
+from ayaka_py_b200.microscale import E2M1, FormatError, Matrix4, Rows8, matrix4, scale_columns
+
+
+def scales_of(exponents):
+    return (torch.as_tensor(exponents) + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+
+
+def random_codes(N, K, seed):
+    gen = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (N, K // 2), generator=gen, dtype=torch.uint8)
+    scales = torch.randint(100, 140, (N, K // 32), generator=gen, dtype=torch.uint8)
+    return codes, scales
+
+
+@pytest.mark.parametrize("N,K", [(1, 32), (5, 96), (128, 128), (129, 160), (300, 1056), (257, 64)])
+def test_layout_of_a_matrix(N, K):
+    codes, scales = random_codes(N, K, N + K)
+    m = Matrix4.from_codes(codes, scales)
+    assert m.shape == (N, K) and m.codes.shape == (-(-N // 128), -(-K // 128), 128, 64) and m.scales.shape == (-(-N // 128), -(-K // 128), 512)
+    back, back_scales = m.row_major()
+    assert torch.equal(back, codes) and torch.equal(back_scales, scales)
+    # the places that the kernels compute: tile, row of the tile, byte; scales at 16 (r % 32) + 4 (r // 32) + block
+    for n, k in {(0, 0), (N - 1, K - 1), (N // 2, K // 3), (N - 1, 0), (0, K - 1)}:
+        byte = m.codes[n // 128, k // 128, n % 128, (k % 128) // 2]
+        assert int(byte) == int(codes[n, k // 2])
+        assert int(m.scales[n // 128, k // 128, (n % 32) * 16 + (n % 128 // 32) * 4 + (k % 128) // 32]) == int(scales[n, k // 32])
+        code = int(codes[n, k // 2]) >> 4 * (k % 2) & 15
+        value = (-1) ** (code >> 3) * E2M1[code & 7] * 2.0 ** (int(scales[n, k // 32]) - 127)
+        assert float(m.decoded()[n, k]) == value
+    # what the last tiles have too much is zeros
+    assert int(m.codes.view(torch.uint8).long().sum()) == int(codes.long().sum())
+    assert int(m.scales.long().sum()) == int(scales.long().sum())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,K", [(3, 64), (130, 288)])
+def test_a_weight_is_rounded_to_the_nearest_codes(dtype, N, K):
+    gen = torch.Generator().manual_seed(K)
+    w = (torch.randn(N, K, generator=gen) * torch.exp(2 * torch.randn(N, 1, generator=gen))).to(dtype)
+    w[0, :32] = 0
+    m = matrix4(w, rows_at_once=64)
+    codes, scales = m.row_major()
+    v = w.double().view(N, -1, 32)
+    s = scales.view(torch.float8_e8m0fnu).double().unsqueeze(-1)
+    largest = v.abs().amax(-1, keepdim=True)
+    assert bool((largest <= 6 * s).all())                                    # nothing is cut off
+    assert bool(((largest > 3 * s) | (largest == 0)).all())                  # and half the scale would be too small
+    assert bool((scales.view(N, -1)[0, 0] == 0)) and bool((m.decoded()[0, :32] == 0).all())
+    grid = torch.tensor(sorted({a for a in E2M1} | {-a for a in E2M1}), dtype=torch.float64)
+    nearest = (v / s).unsqueeze(-1).sub(grid).abs().amin(-1)
+    assert torch.equal((m.decoded().double().view(N, -1, 32) / s - v / s).abs(), nearest)
+
+
+def test_ties_of_a_weight_go_to_the_even_code():
+    """In a block whose scale is 1 (its largest is 6): 0.25 -> 0, 0.75 -> 1, 1.25 -> 1, 1.75 -> 2, 2.5 -> 2, 3.5 -> 4, 5 -> 4."""
+    row = torch.zeros(1, 32)
+    row[0, :8] = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    row[0, 8:16] = -row[0, :8]
+    want = torch.tensor([6.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0])
+    got = matrix4(row).decoded()[0]
+    assert torch.equal(got[:8], want) and torch.equal(got[8:16], -want)
+
+
+def test_a_weight_of_any_strides_and_extremes():
+    w = torch.randn(64, 256, generator=torch.Generator().manual_seed(1))
+    assert torch.equal(matrix4(w.t().contiguous().t()).decoded(), matrix4(w).decoded())
+    assert torch.equal(matrix4(w[:, 64:128]).decoded(), matrix4(w[:, 64:128].contiguous()).decoded())
+    large = torch.full((1, 32), torch.finfo(torch.float32).max)
+    codes, scales = matrix4(large).row_major()
+    assert int(scales) == 126 + 127 and bool((codes == 0x66).all())               # 4 * 2^126: nearly 2^128, rounded up to it
+    small = torch.full((1, 32), 2.0 ** -130)
+    assert torch.equal(matrix4(small).decoded(), torch.zeros(1, 32))               # 2^-130 / 2^-127 = 0.125 -> 0
+
+
+@pytest.mark.parametrize("bad", [
+    lambda: matrix4(torch.zeros(4, 40)), lambda: matrix4(torch.zeros(0, 32)), lambda: matrix4(torch.zeros(2, 32, dtype=torch.float64)),
+    lambda: matrix4(torch.zeros(32)), lambda: matrix4(torch.tensor([[float("nan")] + [0.0] * 31])),
+    lambda: matrix4(torch.tensor([[float("-inf")] + [0.0] * 31])),
+    lambda: Matrix4.from_codes(torch.zeros(4, 16, dtype=torch.int8), torch.zeros(4, 1, dtype=torch.uint8)),
+    lambda: Matrix4.from_codes(torch.zeros(4, 24, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8)),
+    lambda: Matrix4.from_codes(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)),
+    lambda: Matrix4.from_codes(torch.zeros(4, 16, dtype=torch.uint8), torch.full((4, 1), 255, dtype=torch.uint8)),
+    lambda: Matrix4.from_codes(torch.zeros(0, 16, dtype=torch.uint8), torch.zeros(0, 1, dtype=torch.uint8)),
+    lambda: Matrix4(torch.zeros(1, 1, 128, 64, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), (129, 128)),
+    lambda: Rows8(torch.zeros(2, 32), scales_of([[0], [0]])),
+    lambda: Rows8(torch.zeros(2, 48).to(torch.float8_e4m3fn), scales_of([[0], [0]])),
+    lambda: Rows8(torch.zeros(2, 64).to(torch.float8_e4m3fn), scales_of([[0], [0]])),
+    lambda: Rows8(torch.zeros(2, 32).to(torch.float8_e4m3fn), torch.zeros(2, 1, dtype=torch.uint8)),
+    lambda: Rows8(torch.zeros(32).to(torch.float8_e4m3fn), scales_of([[0]])),
+])
+def test_refused_formats(bad):
+    with pytest.raises(FormatError):
+        bad()
+
+
+@pytest.mark.parametrize("T,K", [(0, 32), (1, 32), (3, 96), (5, 512), (2, 544)])
+def test_rows_are_laid_out_as_the_kernels_read_them(T, K):
+    gen = torch.Generator().manual_seed(K)
+    codes = torch.randn(T, K, generator=gen).to(torch.float8_e4m3fn)
+    scales = scales_of(torch.randint(-5, 5, (T, K // 32), generator=gen))
+    wide = torch.zeros(T, K + 5, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    wide[:, 5:].copy_(codes)
+    for c in (codes, wide[:, 5:]):
+        for s in (scales, scales.t().contiguous().t()):
+            rows = Rows8(c, s)
+            assert rows.shape == (T, K) and torch.equal(rows.codes.float(), codes.float()) and torch.equal(rows.scales.float(), scales.float())
+            assert rows.codes.data_ptr() % 16 == 0 and rows.scales.data_ptr() % 4 == 0
+            if T > 1:
+                assert rows.codes.stride(0) % 16 == 0 and rows.scales.stride(0) % 4 == 0
+            want = codes.float() * scales.float().repeat_interleave(32, dim=1)
+            assert torch.equal(rows.decoded(), want)
+    made = Rows8.empty(T, K, "cpu")
+    assert made.shape == (T, K) and made.scales.shape == (T, K // 32) and made.scales.stride(0) == scale_columns(K)
+
+
+# ------------------------------------------------------- refusals of the calls --
+
+class NoLaunch:
+    def __getattr__(self, name):
+        raise AssertionError(f"{name} was reached")
+
+
+def rows_of(T, K):
+    return Rows8(torch.zeros(T, K).to(torch.float8_e4m3fn), scales_of(torch.zeros(T, K // 32)))
+
+
+@pytest.mark.parametrize("call,words", [
+    (lambda: ops.rows8(torch.zeros(2, 40)), "whole blocks"),
+    (lambda: ops.rows8(torch.zeros(2, 0)), "whole blocks"),
+    (lambda: ops.rows8(torch.zeros(64)), "whole blocks"),
+    (lambda: ops.rows8(torch.zeros(64, 32).t().contiguous().t()), "unit column stride"),
+    (lambda: ops.rows8(torch.zeros(2, 32, dtype=torch.float16)), "not supported"),
+    (lambda: ops.rows8(torch.zeros(2, 32)), "current device"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(2, 32, dtype=torch.bfloat16), torch.ones(32), 1e-6), "float32"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(2, 48), torch.ones(48), 1e-6), "whole blocks"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(2, 32), torch.ones(64), 1e-6), "row width"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(2, 32), torch.ones(32, dtype=torch.bfloat16), 1e-6), "float32"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(2, 32), torch.ones(32), 1e-6, torch.zeros(1, 32)), "stream's shape"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(2, 32), torch.ones(32), 1e-6, torch.zeros(2, 32, dtype=torch.float16)), "not supported"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(1, 32).expand(2, 32), torch.ones(32), 1e-6, torch.zeros(2, 32)), "overlap"),
+    (lambda: ops.rmsnorm_rows8(torch.zeros(2, 32), torch.ones(32), 1e-6), "current device"),
+    (lambda: ops.linear4(rows_of(2, 64), matrix4(torch.zeros(8, 32))), "do not fit"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32)), activation="tanh"), "unknown activation"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32)), torch.zeros(7)), "one bias"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32)), torch.zeros(8, dtype=torch.bfloat16)), "float32"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32)), residual=torch.zeros(2, 7)), "output's shape"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32)), out_dtype=torch.float16), "not supported"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32)), out=torch.zeros(2, 8)), "output dtype"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32)), out=torch.zeros(8, 2, dtype=torch.bfloat16).t()), "contiguous"),
+    (lambda: ops.linear4(rows_of(2, 32), matrix4(torch.zeros(8, 32))), "current device"),
+    (lambda: ops.gated_linear4(rows_of(2, 32), matrix4(torch.zeros(32, 32)), matrix4(torch.zeros(64, 32))), "do not fit"),
+    (lambda: ops.gated_linear4(rows_of(2, 64), matrix4(torch.zeros(32, 32)), matrix4(torch.zeros(32, 32))), "do not fit"),
+    (lambda: ops.gated_linear4(rows_of(2, 32), matrix4(torch.zeros(40, 32)), matrix4(torch.zeros(40, 32))), "whole blocks"),
+    (lambda: ops.gated_linear4(rows_of(2, 32), matrix4(torch.zeros(32, 32)), matrix4(torch.zeros(32, 32)), "sigmoid"), "unknown activation"),
+    (lambda: ops.gated_linear4(rows_of(2, 32), matrix4(torch.zeros(32, 32)), matrix4(torch.zeros(32, 32))), "current device"),
+])
+def test_refused_calls(call, words, monkeypatch):
+    """Refused before anything is launched; the last of each operator is a tensor that is not on the current device."""
+    monkeypatch.setattr(ops, "_ready", lambda: NoLaunch())
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    with pytest.raises(ops.KernelError, match=words):
+        call()
