@@ -1,113 +1,440 @@
-// Products of 8-bit rows and 4-bit weights (microscale.cuh), both in blocks of 32 columns that share a power of two:
+// Products of 8-bit rows and 4-bit weights (microscale.cuh), both in blocks of 32 columns that share a power of two, on tcgen05
+// with the scales in tensor memory (kind::mxf8f6f4): nothing is decoded in front of the tensor cores.
 //
 //   linear:  C[t, n] = act(sum_k a[t, k] W[n, k] + bias[n]) (+ residual[t, n])
 //   gated:   rows in 8 bits of act(sum_k a[t, k] G[n, k]) * (sum_k a[t, k] U[n, k])
 //
-// Weights lie in tiles of 128 x 128 (a row of a tile: 64 bytes), their scales beside them as the tensor cores take them.
+// Weights lie in column blocks of 128 (64 bytes of codes a row), their scales beside them as the tensor cores take them.  The
+// copy engine spreads sixteen codes over sixteen bytes on their way into shared memory.
+//
+// Every wait is bounded; one that runs out records a code (101 ... 105) in an error word and the CTA winds down.
+#include <cuda.h>
+
+#include <mutex>
+
 #include "microscale.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
-constexpr int TILE = 128;
-constexpr int FEATURES = 32, TOKENS = 16, THREADS = 256;
+constexpr int BLOCK_K = 128;                    // columns of a stage: 128 bytes a row in shared memory, 64 of a weight's row in memory
+constexpr int TILE_N = 128;                     // features of a CTA
+constexpr int W_BYTES = TILE_N * BLOCK_K;       // a weight tile in shared memory; half of it travels
+constexpr int SCALE_BYTES = 512;                // the scales of 128 rows and four blocks
+constexpr int THREADS = 192;
+constexpr int QUADS = 4;                        // the rows' scales come for four column blocks at a time, into a ring of four such
+constexpr int QUAD_BYTES = 4 * SCALE_BYTES;
 
-struct Matrix {
-  const uint8_t* codes;
-  const uint8_t* scales;
+struct Args {
+  void* C;                       // linear: bfloat16 or float32 [T, N]; gated: codes [T, N]
+  uint8_t* out_scales;           // gated
+  const uint8_t* a_scales;
+  const uint8_t* w_scales[2];
+  const float* bias;
+  const float* residual;
+  int* error;
+  long long a_scale_stride, out_scale_stride;
+  int T, N, K;
+  int n_blocks;                  // the weight's rows in whole 128
+  int act, out_bf16;
 };
 
-__device__ __forceinline__ float e2m1_float(uint32_t code) {
-  const int m = code & 7;
-  const float v = m < 2 ? 0.5f * (float)m : (1.0f + 0.5f * (float)(m & 1)) * (float)(1 << ((m >> 1) - 1));
-  return code & 8 ? -v : v;
+// The scales of row t for column block kb, the first block in the low byte; zeros (2^-127) beyond the matrix.
+__device__ __forceinline__ uint32_t row_scales(const Args& a, int t, int kb) {
+  const int blocks = a.K / MX_BLOCK - 4 * kb;
+  if (t >= a.T || blocks <= 0) return 0u;
+  const uint8_t* at = a.a_scales + (size_t)t * a.a_scale_stride + 4 * kb;
+  if (blocks >= 4) return *reinterpret_cast<const uint32_t*>(at);
+  uint32_t word = at[0];
+  if (blocks > 1) word |= (uint32_t)at[1] << 8;
+  if (blocks > 2) word |= (uint32_t)at[2] << 16;
+  return word;
 }
 
-// A block of 32 features (the lanes) and 16 tokens (two to a warp); K goes by in tiles of 128 columns.
-template <bool GATED>
-__global__ void __launch_bounds__(THREADS)
-linear4_kernel(void* C, uint8_t* out_scales, long long out_scale_stride, const uint8_t* a, long long a_stride, const uint8_t* a_scales,
-               long long a_scale_stride, Matrix m0, Matrix m1, const float* __restrict__ bias, const float* residual, int T, int N, int K,
-               int act, int out_bf16) {
-  __shared__ float at[TOKENS][TILE + 1], wt[GATED ? 2 : 1][FEATURES][TILE + 1];
-  pdl_trigger();
-  pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * FEATURES, t0 = blockIdx.y * TOKENS, n = n0 + lane;
-  const int blocks_k = (K + TILE - 1) / TILE;
-  float sum[GATED ? 2 : 1][2] = {};
-  for (int kb = 0; kb < blocks_k; ++kb) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < TOKENS * TILE; i += THREADS) {
-      const int r = i / TILE, c = i % TILE, t = t0 + r, k = kb * TILE + c;
-      at[r][c] = t < T && k < K ? e4m3_float(a[(size_t)t * a_stride + k]) * mx_scale(a_scales[(size_t)t * a_scale_stride + k / MX_BLOCK]) : 0.f;
+// ---------------------------------------------------------------- few rows --
+// A CTA takes 128 features as the MMA's M side and BT rows as its N side, so that a handful of rows streams every weight byte
+// once; the CTAs of a cluster along z share the tile, each with a part of its column blocks, and exchange their 32-bit sums
+// through shared memory.
+//
+// Warp 0: copies; warp 1: MMA issue, tensor memory; warps 2 ... 5: the rows' scales while the main loop runs, then the epilogue.
+template <int BT, bool GATED>
+struct Few {
+  static constexpr int MATRICES = GATED ? 2 : 1;
+  static constexpr int ROW_BYTES = BT * BLOCK_K;
+  static constexpr int TILE_BYTES = MATRICES * W_BYTES + ROW_BYTES;
+  static constexpr int STAGES = GATED ? (BT <= 16 ? 5 : BT <= 32 ? 4 : 3) : (BT <= 16 ? 5 : BT <= 64 ? (BT <= 32 ? 4 : 6) : 4);
+  static constexpr int TX = MATRICES * (W_BYTES / 2 + SCALE_BYTES) + ROW_BYTES;
+  static constexpr int ACCUMULATORS = MATRICES * BT;
+  static constexpr int SCALE_COLUMNS = 4 * (MATRICES + 1);                   // of a stage
+  static constexpr int USED = ACCUMULATORS + STAGES * SCALE_COLUMNS;
+  static constexpr int TMEM = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+  // shared memory, from a 1024-byte boundary on
+  static constexpr int AT_W_SCALES = STAGES * TILE_BYTES;
+  static constexpr int AT_ROW_SCALES = AT_W_SCALES + STAGES * MATRICES * SCALE_BYTES;
+  static constexpr int AT_BARS = AT_ROW_SCALES + QUADS * QUAD_BYTES;
+  static constexpr int AT_SUMS = AT_BARS + 256;
+  static constexpr int owners(int splits) { return GATED && splits > 4 ? 4 : splits; }       // of a tile's features; a block of 32 has one
+  static constexpr int sums_bytes(int splits) { return MATRICES * splits * (TILE_N / owners(splits)) * BT * 4; }
+  static constexpr int smem(int splits) { return 1024 + AT_SUMS + sums_bytes(splits); }
+};
+
+template <int BT, bool GATED>
+__global__ void __launch_bounds__(THREADS, 1)
+linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
+                   const __grid_constant__ CUtensorMap map_a, const Args args) {
+  using L = Few<BT, GATED>;
+  constexpr int STAGES = L::STAGES, MATRICES = L::MATRICES;
+  constexpr uint32_t IDESC = make_idesc_mx(TILE_N, BT, MX_E2M1, MX_E4M3);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), tiles = (raw + 1023u) & ~1023u;
+  const uint32_t w_scales = tiles + L::AT_W_SCALES, row_ring = tiles + L::AT_ROW_SCALES, bars = tiles + L::AT_BARS, sums = tiles + L::AT_SUMS;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  auto scales_full = [&](int q) { return bars + 8u * (2 * STAGES + q); };
+  auto scales_empty = [&](int q) { return bars + 8u * (2 * STAGES + QUADS + q); };
+  const uint32_t done_bar = bars + 8u * (2 * STAGES + 2 * QUADS), tmem_slot = done_bar + 8u;
+
+  const int warp = warp_number(), lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * TILE_N, t0 = blockIdx.y * BT;
+  const int splits = gridDim.z, z = blockIdx.z;
+  const int total = (args.K + BLOCK_K - 1) / BLOCK_K, base = total / splits, extra = total % splits;
+  const int kb0 = z * base + min(z, extra), num_kb = base + (z < extra ? 1 : 0);      // >= 1 by the host's choice
+
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w0) : "memory");
+    if (GATED) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w1) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
     }
-    for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-      const Matrix m = g ? m1 : m0;
-      const size_t tile = (size_t)(n0 / TILE) * blocks_k + kb;
-      for (int i = threadIdx.x; i < FEATURES * TILE / 2; i += THREADS) {
-        const int r = i / (TILE / 2), c = i % (TILE / 2), tr = n0 % TILE + r;
-        const uint32_t pair = m.codes[(tile * TILE + tr) * (TILE / 2) + c];
-        const float s = mx_scale(m.scales[tile * 512 + (tr % 32) * 16 + (tr / 32) * 4 + c / 16]);
-        wt[g][r][2 * c] = e2m1_float(pair & 15) * s;
-        wt[g][r][2 * c + 1] = e2m1_float(pair >> 4) * s;
+    for (int q = 0; q < QUADS; ++q) {
+      mbar_init(scales_full(q), 1);
+      mbar_init(scales_empty(q), 1);
+    }
+    mbar_init(done_bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(L::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();              // matched by cluster_wait() in every role: nobody sends sums to a CTA that has not started
+  tc_fence_after();
+  const uint32_t tmem = uniform(*(volatile uint32_t*)(smem_raw + (tmem_slot - raw)));
+  pdl_trigger();                 // after the allocation: a successor that is placed early waits for this grid with tensor memory in hand
+
+  bool ok = true;
+  if (warp == 0) {
+    if (elect_one()) {
+      auto load_weights = [&](int i, int s) {
+        const uint32_t at = tiles + s * L::TILE_BYTES;
+        tma_load_3d(at, &map_w0, 0, n0, kb0 + i, full_bar(s));
+        if (GATED) tma_load_3d(at + W_BYTES, &map_w1, 0, n0, kb0 + i, full_bar(s));
+        for (int m = 0; m < MATRICES; ++m)
+          bulk_load(w_scales + (s * MATRICES + m) * SCALE_BYTES, args.w_scales[m] + ((size_t)(kb0 + i) * args.n_blocks + blockIdx.x) * SCALE_BYTES,
+                    SCALE_BYTES, full_bar(s));
+      };
+      auto load_rows = [&](int i, int s) {
+        tma_load_2d(tiles + s * L::TILE_BYTES + MATRICES * W_BYTES, &map_a, (kb0 + i) * BLOCK_K, t0, full_bar(s));
+      };
+      // the weights do not depend on the kernels before this one: their first stages start at once
+      const int pre = min(num_kb, STAGES);
+      for (int i = 0; i < pre; ++i) {
+        mbar_expect_tx(full_bar(i), L::TX);
+        load_weights(i, i);
+      }
+      pdl_wait();
+      for (int i = 0; i < pre; ++i) load_rows(i, i);
+      int issued = pre;
+      for (int i = pre; i < num_kb; ++i) {
+        const int s = i % STAGES;
+        ok = mbar_wait(empty_bar(s), ((uint32_t)(i / STAGES) & 1u) ^ 1u, args.error, 101);
+        if (!ok) break;
+        mbar_expect_tx(full_bar(s), L::TX);
+        load_weights(i, s);
+        load_rows(i, s);
+        issued = i + 1;
+      }
+      if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued
+        for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(full_bar(i % STAGES), (uint32_t)(i / STAGES) & 1u, args.error, 102);
       }
     }
-    __syncthreads();
-    for (int c = 0; c < TILE; ++c)
+    __syncwarp();
+    cluster_wait();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      for (int i = 0; i < num_kb; ++i) {
+        const int s = i % STAGES, q = (i >> 2) % QUADS;
+        if ((i & 3) == 0) ok = mbar_wait(scales_full(q), (uint32_t)(i / (4 * QUADS)) & 1u, args.error, 103);
+        ok = ok && mbar_wait(full_bar(s), (uint32_t)(i / STAGES) & 1u, args.error, 104);
+        if (!ok) break;
+        tc_fence_after();
+        // A stage's scales have columns of their own: by the time the stage comes round again the MMAs that read them are done.
+        const uint32_t columns = tmem + L::ACCUMULATORS + s * L::SCALE_COLUMNS;
+        tmem_cp_scales(columns, make_desc_scales(row_ring + q * QUAD_BYTES + (i & 3) * SCALE_BYTES));
+        for (int m = 0; m < MATRICES; ++m) tmem_cp_scales(columns + 4 * (m + 1), make_desc_scales(w_scales + (s * MATRICES + m) * SCALE_BYTES));
+        const uint32_t at = tiles + s * L::TILE_BYTES;
+        const uint64_t rows = make_desc(at + MATRICES * W_BYTES);
 #pragma unroll
-      for (int g = 0; g < (GATED ? 2 : 1); ++g)
+        for (int k = 0; k < 4; ++k) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sum[g][j] = fmaf(at[warp * 2 + j][c], wt[g][lane][c], sum[g][j]);
+          for (int m = 0; m < MATRICES; ++m)
+            umma_mx(tmem + m * BT, make_desc(at + m * W_BYTES) + (uint64_t)(2 * k), rows + (uint64_t)(2 * k), idesc_mx_block(IDESC, k),
+                    columns + 4 * (m + 1), columns, (i > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(empty_bar(s));
+        if ((i & 3) == 3) umma_commit(scales_empty(q));
+      }
+      umma_commit(done_bar);     // arrives when every MMA issued so far is done
+    }
+    __syncwarp();
+    cluster_wait();
+  } else {
+    const int quarter = warp & 3, e = threadIdx.x - 64, w = warp - 2;
+    pdl_wait();
+    for (int quad = w; quad * 4 < num_kb; quad += 4) {          // quad q is warp q % 4's, and so is its place in the ring
+      uint32_t words[(BT + 31) / 32][4];
+#pragma unroll
+      for (int j = 0; j < (BT + 31) / 32; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = quad * 4 + k, r = 32 * j + lane;
+          words[j][k] = i < num_kb && r < BT ? row_scales(args, t0 + r, kb0 + i) : 0u;
+        }
+      if (quad >= QUADS && !mbar_wait(scales_empty(w), ((uint32_t)(quad / QUADS) & 1u) ^ 1u, args.error, 105)) break;
+#pragma unroll
+      for (int j = 0; j < (BT + 31) / 32; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(row_ring + w * QUAD_BYTES + k * SCALE_BYTES + lane * 16 + j * 4), "r"(words[j][k]) : "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(scales_full(w));
+    }
+    __syncwarp();
+    // Sums go to the CTA that finishes their features, [matrix][split][four rows][feature]: neighbouring lanes 16 bytes apart.
+    const int owners = L::owners(splits), per = TILE_N / owners, local = quarter * 32 + lane;
+    const uint32_t mine = map_to_cta(sums, (uint32_t)(local / per)) + 16u * (uint32_t)(local % per);
+    cluster_wait();
+    ok = mbar_wait(done_bar, 0u, args.error, 106);
+    tc_fence_after();
+#pragma unroll
+    for (int m = 0; m < MATRICES; ++m) {
+      for (int c = 0; c < BT && t0 + c < args.T; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(m * BT + c), r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          st_cluster_v4(mine + 16u * (uint32_t)(((m * splits + z) * (BT / 4) + c / 4 + q) * per), __uint_as_float(r[4 * q]),
+                        __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]));
+      }
+    }
+    tc_fence_before();
+    (void)e;
   }
+  __syncwarp();
+  cluster_sync_all();            // every sum is where it belongs, and nobody leaves before
+
+  if (warp >= 2 && z < L::owners(splits)) {
+    const int owners = L::owners(splits), per = TILE_N / owners;
+    const float4* part = (const float4*)(smem_raw + (sums - raw));
+    for (int p = threadIdx.x - 64; p < per * (BT / 4); p += 128) {
+      const int f = p % per, four = p / per, t = t0 + 4 * four, n = n0 + z * per + f;
+      if (t >= args.T) break;                                    // a warp's lanes have the same four rows where a block's scale is made (per >= 32)
+      float v[MATRICES][4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int t = t0 + warp * 2 + j;
-    if (t >= T) continue;
-    if constexpr (GATED) {
-      const float v = apply_activation(sum[0][j], act) * sum[1][j];      // N is whole blocks of 32
-      const uint32_t code = mx_scale_code(__reduce_max_sync(0xffffffffu, magnitude_bits(v)));
-      ((uint8_t*)C)[(size_t)t * N + n] = (uint8_t)e4m3_pair(v * mx_inverse(code), 0.f);
-      if (lane == 0) out_scales[(size_t)t * out_scale_stride + n0 / MX_BLOCK] = (uint8_t)code;
-    } else if (n < N) {
-      const size_t at_c = (size_t)t * N + n;
-      const float v = apply_activation(sum[0][j] + (bias ? bias[n] : 0.f), act) + (residual ? residual[at_c] : 0.f);
-      if (out_bf16) ((__nv_bfloat16*)C)[at_c] = __float2bfloat16_rn(v);
-      else ((float*)C)[at_c] = v;
+      for (int m = 0; m < MATRICES; ++m) {
+        v[m][0] = v[m][1] = v[m][2] = v[m][3] = 0.f;
+        for (int y = 0; y < splits; ++y) {                       // in the splits' order, whoever came first
+          const float4 x = part[((m * splits + y) * (BT / 4) + four) * per + f];
+          v[m][0] += x.x; v[m][1] += x.y; v[m][2] += x.z; v[m][3] += x.w;
+        }
+      }
+      if constexpr (GATED) {
+        if (n - f % 32 >= args.N) continue;                      // whole blocks of 32 features lie inside or outside
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float y = apply_activation(v[0][u], args.act) * v[MATRICES - 1][u];
+          const uint32_t code = mx_scale_code(__reduce_max_sync(0xffffffffu, magnitude_bits(y)));
+          if (t + u < args.T) {
+            ((uint8_t*)args.C)[(size_t)(t + u) * args.N + n] = (uint8_t)e4m3_pair(y * mx_inverse(code), 0.f);
+            if (lane == 0) args.out_scales[(size_t)(t + u) * args.out_scale_stride + n / MX_BLOCK] = (uint8_t)code;
+          }
+        }
+      } else if (n < args.N) {
+        const float b = args.bias ? args.bias[n] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (t + u >= args.T) break;
+          const size_t at = (size_t)(t + u) * args.N + n;
+          const float y = apply_activation(v[0][u] + b, args.act) + (args.residual ? args.residual[at] : 0.f);
+          if (args.out_bf16) ((__nv_bfloat16*)args.C)[at] = __float2bfloat16_rn(y);
+          else ((float*)args.C)[at] = y;
+        }
+      }
     }
   }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM) : "memory");
 }
 
-int check(const char* name, long long T, int N, int K, int act) {
+// ------------------------------------------------------------------- host --
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn g_encode = nullptr;
+int* g_error_host = nullptr;     // mapped pinned memory: the kernels write, the host reads without a copy
+int* g_error_dev = nullptr;
+std::mutex g_mutex;
+
+int setup() {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (g_encode && g_error_dev) return 0;
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  cudaError_t err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+  if (err != cudaSuccess || fn == nullptr || q != cudaDriverEntryPointSuccess) return ayk_fail("ayk_linear4: cuTensorMapEncodeTiled is not available from this driver");
+  if (!g_error_host) {
+    err = cudaHostAlloc((void**)&g_error_host, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+    if (err != cudaSuccess) return ayk_fail("ayk_linear4: cudaHostAlloc: %s", cudaGetErrorString(err));
+    *g_error_host = 0;
+  }
+  err = cudaHostGetDevicePointer((void**)&g_error_dev, g_error_host, 0);
+  if (err != cudaSuccess) return ayk_fail("ayk_linear4: cudaHostGetDevicePointer: %s", cudaGetErrorString(err));
+  g_encode = (EncodeTiledFn)fn;
+  return 0;
+}
+
+// Rows of codes [T, K], rows `stride` bytes apart: boxes of 128 columns.
+int encode_rows(CUtensorMap* map, const void* p, long long T, int K, long long stride, int box) {
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)T}, strides[1] = {(cuuint64_t)stride};
+  cuuint32_t boxes[2] = {BLOCK_K, (cuuint32_t)box}, step[2] = {1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return ayk_fail("ayk_linear4: cuTensorMapEncodeTiled of the rows failed with %d", (int)r);
+  return 0;
+}
+// A weight's codes [K / 128][rows][128]: boxes of `box` rows, spread to a byte each.
+int encode_weight(CUtensorMap* map, const void* p, int rows, int K, int box) {
+  cuuint64_t dims[3] = {BLOCK_K, (cuuint64_t)rows, (cuuint64_t)((K + BLOCK_K - 1) / BLOCK_K)};
+  cuuint64_t strides[2] = {BLOCK_K / 2, (cuuint64_t)rows * (BLOCK_K / 2)};
+  cuuint32_t boxes[3] = {BLOCK_K, (cuuint32_t)box, 1}, step[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, const_cast<void*>(p), dims, strides, boxes, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return ayk_fail("ayk_linear4: cuTensorMapEncodeTiled of the weight failed with %d", (int)r);
+  return 0;
+}
+
+// CTAs along K: as many as keep every multiprocessor's two places filled, with four column blocks for each at least.
+int few_splits(int tiles, int blocks_k, int most) {
+  int s = 1;
+  while (2 * s <= most && tiles * 2 * s <= 2 * ayk_sm_count() && blocks_k >= 4 * 2 * s) s *= 2;
+  return s;
+}
+
+template <int BT, bool GATED>
+int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& a, const Args& args, const char* name, cudaStream_t stream) {
+  using L = Few<BT, GATED>;
+  constexpr int MOST = GATED && BT >= 64 ? 4 : 8;                // splits; what their sums leave of shared memory
+  static_assert(L::smem(MOST) <= 232448 && L::smem(1) <= 232448, "shared memory");
+  static_assert(L::USED <= 512 && 8 * (2 * L::STAGES + 2 * QUADS + 2) <= 256 && L::AT_BARS % 16 == 0, "layout");
+  const int tiles_n = (args.N + TILE_N - 1) / TILE_N, tiles_t = (args.T + BT - 1) / BT;
+  AYK_REQUIRE(tiles_t <= 65535, "%s: too many rows (%d)", name, args.T);
+  const int splits = few_splits(tiles_n * tiles_t, (args.K + BLOCK_K - 1) / BLOCK_K, MOST);
+  static AykPerDevice configured;
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    bool& done = configured.here();
+    if (!done) {
+      const int most = L::smem(MOST) > L::smem(1) ? L::smem(MOST) : L::smem(1);
+      const cudaError_t err = cudaFuncSetAttribute(linear4_few_kernel<BT, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (err != cudaSuccess) return ayk_fail("%s: shared memory %d: %s", name, most, cudaGetErrorString(err));
+      done = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles_n, tiles_t, splits);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = L::smem(splits);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = splits;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ayk_pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, linear4_few_kernel<BT, GATED>, w0, w1, a, args);
+  return ayk_check_launch(name);
+}
+
+int check(const char* name, const void* a, long long a_stride, const void* a_scales, long long a_scale_stride, long long T, int N, int K, int act) {
   AYK_REQUIRE(N > 0 && K > 0 && K % MX_BLOCK == 0, "%s: a product of %d columns over rows of %d (whole blocks of %d)", name, N, K, MX_BLOCK);
-  AYK_REQUIRE(T >= 0 && T <= 65535ll * TOKENS, "%s: too many rows (%lld)", name, T);
+  AYK_REQUIRE(T >= 0 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256, "%s: too many rows (%lld) or columns (%d)", name, T, N);
   AYK_REQUIRE(act >= AYK_ACT_NONE && act <= AYK_ACT_SILU, "%s: unknown activation %d", name, act);
+  AYK_REQUIRE((uintptr_t)a % 16 == 0 && a_stride % 16 == 0 && a_stride >= K, "%s: rows of codes must lie on 16-byte boundaries", name);
+  AYK_REQUIRE((uintptr_t)a_scales % 4 == 0 && (T <= 1 || a_scale_stride % 4 == 0), "%s: rows of scales must lie on 4-byte boundaries", name);
   return 0;
 }
 
 }  // namespace
 
+AYK_EXPORT int ayk_linear4_error() { return g_error_host ? *g_error_host : 0; }
+AYK_EXPORT void ayk_linear4_clear_error() { if (g_error_host) *g_error_host = 0; }
+
+// a [T, K] e4m3 (rows a_stride bytes apart) and its scales; codes and scales of the weight [N, K] as laid out (see the head); C
+// [T, N] float32 or bfloat16; bias, residual float32 or null (the residual may be a float32 C).
 AYK_EXPORT int ayk_linear4(void* C, const void* a, long long a_stride, const void* a_scales, long long a_scale_stride, const void* codes,
                            const void* scales, const float* bias, const float* residual, long long T, int N, int K, int act, int out_dtype,
                            cudaStream_t stream) {
-  if (check("ayk_linear4", T, N, K, act) != 0) return -1;
+  if (check("ayk_linear4", a, a_stride, a_scales, a_scale_stride, T, N, K, act) != 0) return -1;
   AYK_REQUIRE(out_dtype == AYK_DTYPE_F32 || out_dtype == AYK_DTYPE_BF16, "ayk_linear4: unknown output dtype %d", out_dtype);
   if (T == 0) return 0;
-  const Matrix m{(const uint8_t*)codes, (const uint8_t*)scales};
-  ayk_launch(linear4_kernel<false>, dim3((N + FEATURES - 1) / FEATURES, (unsigned)((T + TOKENS - 1) / TOKENS)), dim3(THREADS), 0, stream, C,
-             (uint8_t*)nullptr, 0ll, (const uint8_t*)a, a_stride, (const uint8_t*)a_scales, a_scale_stride, m, m, bias, residual, (int)T, N, K,
-             act, out_dtype == AYK_DTYPE_BF16);
-  return ayk_check_launch("ayk_linear4");
+  if (setup() != 0) return -1;
+  Args args{};
+  args.C = C; args.a_scales = (const uint8_t*)a_scales; args.a_scale_stride = a_scale_stride; args.w_scales[0] = (const uint8_t*)scales;
+  args.bias = bias; args.residual = residual; args.error = g_error_dev; args.T = (int)T; args.N = N; args.K = K;
+  args.n_blocks = (N + TILE_N - 1) / TILE_N; args.act = act; args.out_bf16 = out_dtype == AYK_DTYPE_BF16;
+  const int bt = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  CUtensorMap mw, ma;
+  if (encode_weight(&mw, codes, args.n_blocks * TILE_N, K, TILE_N) != 0 || encode_rows(&ma, a, T, K, a_stride, bt) != 0) return -1;
+  switch (bt) {
+    case 16: return launch_few<16, false>(mw, mw, ma, args, "ayk_linear4", stream);
+    case 32: return launch_few<32, false>(mw, mw, ma, args, "ayk_linear4", stream);
+    case 64: return launch_few<64, false>(mw, mw, ma, args, "ayk_linear4", stream);
+    default: return launch_few<128, false>(mw, mw, ma, args, "ayk_linear4", stream);
+  }
 }
 
+// out [T, N] e4m3 and out_scales (rows out_scale_stride bytes apart) of act(a gate^T) * (a up^T).
 AYK_EXPORT int ayk_gated_linear4(void* out, void* out_scales, long long out_scale_stride, const void* a, long long a_stride, const void* a_scales,
                                  long long a_scale_stride, const void* gate_codes, const void* gate_scales, const void* up_codes,
                                  const void* up_scales, long long T, int N, int K, int act, cudaStream_t stream) {
-  if (check("ayk_gated_linear4", T, N, K, act) != 0) return -1;
+  if (check("ayk_gated_linear4", a, a_stride, a_scales, a_scale_stride, T, N, K, act) != 0) return -1;
   AYK_REQUIRE(N % MX_BLOCK == 0, "ayk_gated_linear4: a row of %d is not whole blocks of %d", N, MX_BLOCK);
   if (T == 0) return 0;
-  const Matrix g{(const uint8_t*)gate_codes, (const uint8_t*)gate_scales}, u{(const uint8_t*)up_codes, (const uint8_t*)up_scales};
-  ayk_launch(linear4_kernel<true>, dim3(N / FEATURES, (unsigned)((T + TOKENS - 1) / TOKENS)), dim3(THREADS), 0, stream, out,
-             (uint8_t*)out_scales, out_scale_stride, (const uint8_t*)a, a_stride, (const uint8_t*)a_scales, a_scale_stride, g, u,
-             (const float*)nullptr, (const float*)nullptr, (int)T, N, K, act, 0);
-  return ayk_check_launch("ayk_gated_linear4");
+  if (setup() != 0) return -1;
+  Args args{};
+  args.C = out; args.out_scales = (uint8_t*)out_scales; args.out_scale_stride = out_scale_stride;
+  args.a_scales = (const uint8_t*)a_scales; args.a_scale_stride = a_scale_stride;
+  args.w_scales[0] = (const uint8_t*)gate_scales; args.w_scales[1] = (const uint8_t*)up_scales; args.error = g_error_dev;
+  args.T = (int)T; args.N = N; args.K = K; args.n_blocks = (N + TILE_N - 1) / TILE_N; args.act = act;
+  const int bt = T <= 16 ? 16 : T <= 32 ? 32 : 64;
+  CUtensorMap mg, mu, ma;
+  if (encode_weight(&mg, gate_codes, args.n_blocks * TILE_N, K, TILE_N) != 0 || encode_weight(&mu, up_codes, args.n_blocks * TILE_N, K, TILE_N) != 0 ||
+      encode_rows(&ma, a, T, K, a_stride, bt) != 0)
+    return -1;
+  switch (bt) {
+    case 16: return launch_few<16, true>(mg, mu, ma, args, "ayk_gated_linear4", stream);
+    case 32: return launch_few<32, true>(mg, mu, ma, args, "ayk_gated_linear4", stream);
+    default: return launch_few<64, true>(mg, mu, ma, args, "ayk_gated_linear4", stream);
+  }
 }

@@ -99,6 +99,12 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
                ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
+// `bytes` (whole 16) side by side, both addresses on 16-byte boundaries.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 // -------------------------------------------------------------- tcgen05.mma --
 // Shared-memory matrix descriptor, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024
 // bytes apart (stride byte offset), version 1 (sm_100).  The same bits describe a K-major
@@ -136,6 +142,30 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// kind::mxf8f6f4, blocks of 32 columns of K with an e8m0 scale each: 8-bit containers in shared memory (of e2m1, eight bytes of
+// codes and eight that are not looked at for every sixteen numbers), D float32, K = 32 to an instruction.  Scales lie in tensor
+// memory: row r's for four blocks of K in the four bytes of column r / 32, lane r % 32, the same in each quarter of the lanes;
+// `block` says which byte.
+constexpr uint32_t MX_E4M3 = 0, MX_E2M1 = 5;
+__host__ __device__ constexpr uint32_t make_idesc_mx(int m, int n, uint32_t a_type, uint32_t b_type) {
+  return (a_type << 7) | (b_type << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27);
+}
+__host__ __device__ constexpr uint32_t idesc_mx_block(uint32_t idesc, int block) { return idesc | ((uint32_t)block << 4) | ((uint32_t)block << 29); }
+__device__ __forceinline__ void umma_mx(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t scales_a, uint32_t scales_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(scales_a), "r"(scales_b), "r"(accumulate) : "memory");
+}
+// The scales of 128 rows, 512 bytes of shared memory (16 (r % 32) + 4 (r / 32) + block), to four columns of tensor memory, in all
+// four quarters of the lanes; in order with the MMAs that the same thread issues after it.
+__device__ __forceinline__ uint64_t make_desc_scales(uint32_t addr) {      // no swizzle: 8 rows of 16 bytes side by side, the next 8 behind them
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 // arrives at the barrier once every MMA issued so far by this thread is done
 __device__ __forceinline__ void umma_commit(uint32_t bar) {

@@ -14,7 +14,7 @@ import torch
 
 BLOCK = 32                                       # columns that share a scale
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)  # magnitudes of the codes 0 ... 7; 8 ... 15 are their negatives
-TILE = 128                                       # rows, and columns, of a tile of a laid-out matrix
+TILE = 128                                       # columns of a block of a laid-out matrix; its rows are whole tiles of as many
 
 
 class FormatError(ValueError):
@@ -66,20 +66,21 @@ class Rows8:
 
 
 class Matrix4:
-    """A weight [N, K] of e2m1 codes with a scale for every 32 columns, laid out once for the kernels: tiles of 128 rows and 128
-    columns lie one behind the other (along K first), a tile's row as 64 bytes (two codes to a byte, the even column in the low
-    half), a tile's 128 x 4 scales as the tensor cores take them (row r, block b at byte 16 (r % 32) + 4 (r // 32) + b).
-    What a last tile has too much is zeros.  Made by ``Matrix4.from_codes`` or ``matrix4``."""
+    """A weight [N, K] of e2m1 codes with a scale for every 32 columns, laid out once for the kernels: column blocks of 128 one
+    behind the other, in each the rows (rounded up to whole 128) as 64 bytes (two codes to a byte, the even column in the low
+    half); and for every column block and 128 rows the 128 x 4 scales as the tensor cores take them (row r, block b at byte
+    16 (r % 32) + 4 (r // 32) + b).  What the last blocks have too much is zeros.  Made by ``Matrix4.from_codes`` or ``matrix4``
+    and complete in memory by then: the kernels may read it ahead of earlier work in their stream, so it is not written to again."""
 
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int]):
         N, K = shape
-        tiles = -(-N // TILE), -(-K // TILE)
-        if (tuple(codes.shape) != (*tiles, TILE, TILE // 2) or codes.dtype != torch.uint8 or not codes.is_contiguous()
-                or tuple(scales.shape) != (*tiles, TILE * TILE // BLOCK) or scales.dtype != torch.uint8 or not scales.is_contiguous()
-                or N < 1 or K < BLOCK or K % BLOCK or codes.device != scales.device):
-            raise FormatError(f"not the tiles of a weight {tuple(shape)}: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
+        nt, kt = -(-N // TILE), -(-K // TILE)
+        if (tuple(codes.shape) != (kt, nt * TILE, TILE // 2) or codes.dtype != torch.uint8 or not codes.is_contiguous()
+                or tuple(scales.shape) != (kt, nt, TILE * TILE // BLOCK) or scales.dtype != torch.uint8 or not scales.is_contiguous()
+                or N < 1 or K < BLOCK or K % BLOCK or codes.device != scales.device or codes.data_ptr() % 32 or scales.data_ptr() % 16):
+            raise FormatError(f"not the blocks of a weight {tuple(shape)}: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
         self.codes, self.scales, self.shape = codes, scales, (int(N), int(K))
 
     @classmethod
@@ -100,15 +101,17 @@ class Matrix4:
         c[:N, :K // 2] = codes
         s = torch.zeros((nt * TILE, kt * TILE // BLOCK), dtype=torch.uint8, device=codes.device)
         s[:N, :K // BLOCK] = scales
-        c = c.view(nt, TILE, kt, TILE // 2).transpose(1, 2).contiguous()
-        s = s.view(nt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).contiguous().view(nt, kt, TILE * TILE // BLOCK)
+        c = c.view(nt * TILE, kt, TILE // 2).transpose(0, 1).clone(memory_format=torch.contiguous_format)
+        s = s.view(nt, 4, 32, kt, 4).permute(3, 0, 2, 1, 4).clone(memory_format=torch.contiguous_format).view(kt, nt, TILE * TILE // BLOCK)
+        if c.is_cuda:
+            torch.cuda.current_stream(c.device).synchronize()
         return cls(c, s, (N, K))
 
     def row_major(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(codes, scales as uint8), as ``from_codes`` takes them."""
-        (N, K), (nt, kt) = self.shape, self.codes.shape[:2]
-        codes = self.codes.transpose(1, 2).reshape(nt * TILE, kt * TILE // 2)[:N, :K // 2]
-        scales = self.scales.view(nt, kt, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(nt * TILE, kt * TILE // BLOCK)[:N, :K // BLOCK]
+        (N, K), (kt, nt) = self.shape, self.scales.shape[:2]
+        codes = self.codes.transpose(0, 1).reshape(nt * TILE, kt * TILE // 2)[:N, :K // 2]
+        scales = self.scales.view(kt, nt, 32, 4, 4).permute(1, 3, 2, 0, 4).reshape(nt * TILE, kt * TILE // BLOCK)[:N, :K // BLOCK]
         return codes.contiguous(), scales.contiguous()
 
     def decoded(self) -> torch.Tensor:

@@ -23,18 +23,18 @@ def random_codes(N, K, seed):
 def test_layout_of_a_matrix(N, K):
     codes, scales = random_codes(N, K, N + K)
     m = Matrix4.from_codes(codes, scales)
-    assert m.shape == (N, K) and m.codes.shape == (-(-N // 128), -(-K // 128), 128, 64) and m.scales.shape == (-(-N // 128), -(-K // 128), 512)
+    assert m.shape == (N, K) and m.codes.shape == (-(-K // 128), -(-N // 128) * 128, 64) and m.scales.shape == (-(-K // 128), -(-N // 128), 512)
     back, back_scales = m.row_major()
     assert torch.equal(back, codes) and torch.equal(back_scales, scales)
-    # the places that the kernels compute: tile, row of the tile, byte; scales at 16 (r % 32) + 4 (r // 32) + block
+    # the places that the kernels compute: column block, row, byte; scales at 16 (r % 32) + 4 (r // 32) + block
     for n, k in {(0, 0), (N - 1, K - 1), (N // 2, K // 3), (N - 1, 0), (0, K - 1)}:
-        byte = m.codes[n // 128, k // 128, n % 128, (k % 128) // 2]
+        byte = m.codes[k // 128, n, (k % 128) // 2]
         assert int(byte) == int(codes[n, k // 2])
-        assert int(m.scales[n // 128, k // 128, (n % 32) * 16 + (n % 128 // 32) * 4 + (k % 128) // 32]) == int(scales[n, k // 32])
+        assert int(m.scales[k // 128, n // 128, (n % 32) * 16 + (n % 128 // 32) * 4 + (k % 128) // 32]) == int(scales[n, k // 32])
         code = int(codes[n, k // 2]) >> 4 * (k % 2) & 15
         value = (-1) ** (code >> 3) * E2M1[code & 7] * 2.0 ** (int(scales[n, k // 32]) - 127)
         assert float(m.decoded()[n, k]) == value
-    # what the last tiles have too much is zeros
+    # what the last blocks have too much is zeros
     assert int(m.codes.view(torch.uint8).long().sum()) == int(codes.long().sum())
     assert int(m.scales.long().sum()) == int(scales.long().sum())
 
@@ -88,7 +88,7 @@ def test_a_weight_of_any_strides_and_extremes():
     lambda: Matrix4.from_codes(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)),
     lambda: Matrix4.from_codes(torch.zeros(4, 16, dtype=torch.uint8), torch.full((4, 1), 255, dtype=torch.uint8)),
     lambda: Matrix4.from_codes(torch.zeros(0, 16, dtype=torch.uint8), torch.zeros(0, 1, dtype=torch.uint8)),
-    lambda: Matrix4(torch.zeros(1, 1, 128, 64, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), (129, 128)),
+    lambda: Matrix4(torch.zeros(1, 128, 64, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), (129, 128)),
     lambda: Rows8(torch.zeros(2, 32), scales_of([[0], [0]])),
     lambda: Rows8(torch.zeros(2, 48).to(torch.float8_e4m3fn), scales_of([[0], [0]])),
     lambda: Rows8(torch.zeros(2, 64).to(torch.float8_e4m3fn), scales_of([[0], [0]])),
