@@ -7,10 +7,11 @@
 // Weights lie in column blocks of 128 (64 bytes of codes a row), their scales beside them as the tensor cores take them.  The
 // copy engine spreads sixteen codes over sixteen bytes on their way into shared memory.
 //
-// Every wait is bounded; one that runs out records a code (101 ... 105) in an error word and the CTA winds down.
+// Every wait is bounded; one that runs out records a code (101 ... 118) in an error word and the CTA winds down.
 #include <cuda.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "microscale.cuh"
 #include "tcgen05.cuh"
@@ -21,7 +22,6 @@ constexpr int BLOCK_K = 128;                    // columns of a stage: 128 bytes
 constexpr int TILE_N = 128;                     // features of a CTA
 constexpr int W_BYTES = TILE_N * BLOCK_K;       // a weight tile in shared memory; half of it travels
 constexpr int SCALE_BYTES = 512;                // the scales of 128 rows and four blocks
-constexpr int THREADS = 192;
 constexpr int QUADS = 4;                        // the rows' scales come for four column blocks at a time, into a ring of four such
 constexpr int QUAD_BYTES = 4 * SCALE_BYTES;
 
@@ -51,18 +51,63 @@ __device__ __forceinline__ uint32_t row_scales(const Args& a, int t, int kb) {
   return word;
 }
 
+// One feature n (a lane's) of CNT rows from t on.  Linear: bias, activation, residual (every load before the first store: the
+// residual may be C), rounding.  Gated: the warp's 32 features are a block, whose largest magnitude makes the scale.
+// `inside`: n is a feature (of a gated product all 32 or none).
+template <bool GATED, int ACT, int CNT>
+__device__ __forceinline__ void finish_rows(const Args& a, int t, int n, bool inside, const float (&v)[CNT], const float (&u)[CNT]) {
+  if constexpr (GATED) {
+#pragma unroll
+    for (int j = 0; j < CNT; ++j) {
+      const float y = apply_activation_tc<ACT>(v[j], a.act) * u[j];
+      const uint32_t code = mx_scale_code(__reduce_max_sync(0xffffffffu, magnitude_bits(y)));
+      if (inside && t + j < a.T) {
+        ((uint8_t*)a.C)[(size_t)(t + j) * a.N + n] = (uint8_t)e4m3_pair(y * mx_inverse(code), 0.f);
+        if ((threadIdx.x & 31) == 0) a.out_scales[(size_t)(t + j) * a.out_scale_stride + n / MX_BLOCK] = (uint8_t)code;
+      }
+    }
+  } else if (inside) {
+    const float b = a.bias ? a.bias[n] : 0.f;
+    float r[CNT];
+#pragma unroll
+    for (int j = 0; j < CNT; ++j) r[j] = a.residual && t + j < a.T ? a.residual[(size_t)(t + j) * a.N + n] : 0.f;
+#pragma unroll
+    for (int j = 0; j < CNT; ++j) {
+      if (t + j < a.T) {
+        const float y = apply_activation_tc<ACT>(v[j] + b, a.act) + r[j];
+        const size_t at = (size_t)(t + j) * a.N + n;
+        if (a.out_bf16) ((__nv_bfloat16*)a.C)[at] = __float2bfloat16_rn(y);
+        else ((float*)a.C)[at] = y;
+      }
+    }
+  }
+}
+
+// The activation as a constant of the code that `run` is compiled to; the ones that few products use share one copy.
+template <typename Run>
+__device__ __forceinline__ void with_activation(int act, Run run) {
+  if (act == AYK_ACT_NONE) run(std::integral_constant<int, AYK_ACT_NONE>());
+  else if (act == AYK_ACT_SILU) run(std::integral_constant<int, AYK_ACT_SILU>());
+  else if (act == AYK_ACT_GELU_TANH) run(std::integral_constant<int, AYK_ACT_GELU_TANH>());
+  else run(std::integral_constant<int, -1>());
+}
+
 // ---------------------------------------------------------------- few rows --
 // A CTA takes 128 features as the MMA's M side and BT rows as its N side, so that a handful of rows streams every weight byte
 // once; the CTAs of a cluster along z share the tile, each with a part of its column blocks, and exchange their 32-bit sums
 // through shared memory.
 //
-// Warp 0: copies; warp 1: MMA issue, tensor memory; warps 2 ... 5: the rows' scales while the main loop runs, then the epilogue.
+// Warp 0: copies; warp 1: MMA issue, tensor memory; warps 2 ... 5 (64 rows: 2 ... 9): the rows' scales while the main loop runs,
+// then the epilogue.
 template <int BT, bool GATED>
 struct Few {
   static constexpr int MATRICES = GATED ? 2 : 1;
   static constexpr int ROW_BYTES = BT * BLOCK_K;
   static constexpr int TILE_BYTES = MATRICES * W_BYTES + ROW_BYTES;
-  static constexpr int STAGES = GATED ? (BT <= 16 ? 5 : BT <= 32 ? 4 : 3) : (BT <= 16 ? 5 : BT <= 64 ? (BT <= 32 ? 4 : 6) : 4);
+  static constexpr int STAGES = GATED ? (BT <= 16 ? 5 : BT <= 32 ? 4 : 3) : (BT <= 16 ? 5 : BT <= 32 ? 4 : 6);
+  static constexpr int PLACES = GATED || BT > 32 ? 1 : 2;                    // CTAs that a multiprocessor's shared memory holds
+  static constexpr int EPILOGUE = BT <= 32 ? 128 : 256;                      // threads
+  static constexpr int THREADS = 64 + EPILOGUE;
   static constexpr int TX = MATRICES * (W_BYTES / 2 + SCALE_BYTES) + ROW_BYTES;
   static constexpr int ACCUMULATORS = MATRICES * BT;
   static constexpr int SCALE_COLUMNS = 4 * (MATRICES + 1);                   // of a stage
@@ -79,7 +124,7 @@ struct Few {
 };
 
 template <int BT, bool GATED>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Few<BT, GATED>::THREADS, 1)
 linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                    const __grid_constant__ CUtensorMap map_a, const Args args) {
   using L = Few<BT, GATED>;
@@ -194,9 +239,9 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
     __syncwarp();
     cluster_wait();
   } else {
-    const int quarter = warp & 3, e = threadIdx.x - 64, w = warp - 2;
+    const int quarter = warp & 3, w = warp - 2;
     pdl_wait();
-    for (int quad = w; quad * 4 < num_kb; quad += 4) {          // quad q is warp q % 4's, and so is its place in the ring
+    for (int quad = w; w < QUADS && quad * 4 < num_kb; quad += 4) {          // quad q is warp q % 4's, and so is its place in the ring
       uint32_t words[(BT + 31) / 32][4];
 #pragma unroll
       for (int j = 0; j < (BT + 31) / 32; ++j)
@@ -216,72 +261,386 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
       if (lane == 0) mbar_arrive(scales_full(w));
     }
     __syncwarp();
-    // Sums go to the CTA that finishes their features, [matrix][split][four rows][feature]: neighbouring lanes 16 bytes apart.
-    const int owners = L::owners(splits), per = TILE_N / owners, local = quarter * 32 + lane;
-    const uint32_t mine = map_to_cta(sums, (uint32_t)(local / per)) + 16u * (uint32_t)(local % per);
     cluster_wait();
     ok = mbar_wait(done_bar, 0u, args.error, 106);
     tc_fence_after();
+    const uint32_t quarter_at = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int first = 16 * (w / 4), step = L::EPILOGUE / 8;       // two warps to a quarter of the features: every other 16 rows each
+    if (splits == 1) {
+      const int n = n0 + quarter * 32 + lane;
+      with_activation(args.act, [&](auto act) {
+#pragma unroll 1
+        for (int c = first; c < BT && t0 + c < args.T; c += step) {
+          uint32_t r[MATRICES][16];
 #pragma unroll
-    for (int m = 0; m < MATRICES; ++m) {
-      for (int c = 0; c < BT && t0 + c < args.T; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(m * BT + c), r);
-        tmem_ld_wait();
+          for (int m = 0; m < MATRICES; ++m) tmem_ld16(quarter_at + (uint32_t)(m * BT + c), r[m]);
+          tmem_ld_wait();
+          float v[MATRICES][16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          st_cluster_v4(mine + 16u * (uint32_t)(((m * splits + z) * (BT / 4) + c / 4 + q) * per), __uint_as_float(r[4 * q]),
-                        __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]));
-      }
-    }
-    tc_fence_before();
-    (void)e;
-  }
-  __syncwarp();
-  cluster_sync_all();            // every sum is where it belongs, and nobody leaves before
-
-  if (warp >= 2 && z < L::owners(splits)) {
-    const int owners = L::owners(splits), per = TILE_N / owners;
-    const float4* part = (const float4*)(smem_raw + (sums - raw));
-    for (int p = threadIdx.x - 64; p < per * (BT / 4); p += 128) {
-      const int f = p % per, four = p / per, t = t0 + 4 * four, n = n0 + z * per + f;
-      if (t >= args.T) break;                                    // a warp's lanes have the same four rows where a block's scale is made (per >= 32)
-      float v[MATRICES][4];
+          for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[m][j] = __uint_as_float(r[m][j]);
+          finish_rows<GATED, decltype(act)::value, 16>(args, t0 + c, n, n < args.N, v[0], v[MATRICES - 1]);
+        }
+      });
+    } else {
+      // Sums go to the CTA that finishes their features, [matrix][split][four rows][feature]: neighbouring lanes 16 bytes apart.
+      const int per = TILE_N / L::owners(splits), local = quarter * 32 + lane;
+      const uint32_t mine = map_to_cta(sums, (uint32_t)(local / per)) + 16u * (uint32_t)(local % per);
 #pragma unroll
       for (int m = 0; m < MATRICES; ++m) {
-        v[m][0] = v[m][1] = v[m][2] = v[m][3] = 0.f;
-        for (int y = 0; y < splits; ++y) {                       // in the splits' order, whoever came first
-          const float4 x = part[((m * splits + y) * (BT / 4) + four) * per + f];
-          v[m][0] += x.x; v[m][1] += x.y; v[m][2] += x.z; v[m][3] += x.w;
+#pragma unroll 1
+        for (int c = first; c < BT && t0 + c < args.T; c += step) {
+          uint32_t r[16];
+          tmem_ld16(quarter_at + (uint32_t)(m * BT + c), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            st_cluster_v4(mine + 16u * (uint32_t)(((m * splits + z) * (BT / 4) + c / 4 + q) * per), __uint_as_float(r[4 * q]),
+                          __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]));
         }
       }
-      if constexpr (GATED) {
-        if (n - f % 32 >= args.N) continue;                      // whole blocks of 32 features lie inside or outside
+    }
+  }
+  __syncwarp();
+  if (splits > 1) {
+    cluster_sync_all();          // every sum is where it belongs, and nobody leaves before
+    if (warp >= 2 && z < L::owners(splits)) {
+      const int per = TILE_N / L::owners(splits);
+      const float4* part = (const float4*)(smem_raw + (sums - raw));
+      with_activation(args.act, [&](auto act) {
+#pragma unroll 1
+        for (int p = threadIdx.x - 64; p < per * (BT / 4); p += L::EPILOGUE) {
+          const int f = p % per, four = p / per, t = t0 + 4 * four, n = n0 + z * per + f;
+          if (t >= args.T) break;              // a warp's lanes have the same four rows where a block's scale is made (per >= 32)
+          float v[MATRICES][4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float y = apply_activation(v[0][u], args.act) * v[MATRICES - 1][u];
-          const uint32_t code = mx_scale_code(__reduce_max_sync(0xffffffffu, magnitude_bits(y)));
-          if (t + u < args.T) {
-            ((uint8_t*)args.C)[(size_t)(t + u) * args.N + n] = (uint8_t)e4m3_pair(y * mx_inverse(code), 0.f);
-            if (lane == 0) args.out_scales[(size_t)(t + u) * args.out_scale_stride + n / MX_BLOCK] = (uint8_t)code;
+          for (int m = 0; m < MATRICES; ++m) {
+            const float4* at = part + ((size_t)m * splits * (BT / 4) + four) * per + f;
+            v[m][0] = v[m][1] = v[m][2] = v[m][3] = 0.f;
+#pragma unroll 1
+            for (int y = 0; y < splits; y += 2) {                // in the splits' order, whoever came first
+              const float4 x0 = at[y * (BT / 4) * per], x1 = at[(y + 1) * (BT / 4) * per];
+              v[m][0] += x0.x; v[m][1] += x0.y; v[m][2] += x0.z; v[m][3] += x0.w;
+              v[m][0] += x1.x; v[m][1] += x1.y; v[m][2] += x1.z; v[m][3] += x1.w;
+            }
           }
+          finish_rows<GATED, decltype(act)::value, 4>(args, t, n, n < args.N, v[0], v[MATRICES - 1]);
         }
-      } else if (n < args.N) {
-        const float b = args.bias ? args.bias[n] : 0.f;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (t + u >= args.T) break;
-          const size_t at = (size_t)(t + u) * args.N + n;
-          const float y = apply_activation(v[0][u] + b, args.act) + (args.residual ? args.residual[at] : 0.f);
-          if (args.out_bf16) ((__nv_bfloat16*)args.C)[at] = __float2bfloat16_rn(y);
-          else ((float*)args.C)[at] = y;
-        }
-      }
+      });
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM) : "memory");
+}
+
+// --------------------------------------------------------------- many rows --
+// Persistent CTAs over tiles of 128 rows (the MMA's M side, a row to a lane of tensor memory) by BN features (its N side; of a
+// gated product BN of each matrix), two accumulators in tensor memory so that a tile's epilogue runs under the next one's main
+// loop.  An epilogue thread owns a row and stores runs of features.
+//
+// Warp 0: copies; warp 1: MMA issue, tensor memory; warp 2: the rows' scales; warp 3: the weights', which it shifts so that a tile's
+// first feature has the first column (the MMA wants its scales from a whole group of four columns on, and a tile may start at any
+// 32 features); warps 4 ... 11: epilogue, two to a quarter of the rows, each with every other run of features.
+constexpr int TILE_T = 128;
+constexpr int MANY_THREADS = 384;
+constexpr int ROWS_BYTES = TILE_T * BLOCK_K;
+constexpr int MANY_MOST_STAGES = 8;
+constexpr int MANY_QUADS = 3;                   // scales come for four column blocks at a time, into a ring of three such
+constexpr int MANY_MOST_BLOCKS = 3;             // of 128 features' scales that a tile of 224 touches
+
+struct ManyShape {
+  int BN, stages, m_tiles, n_tiles;
+  int w_blocks;                  // groups of 128 features in a tile, the last one not full perhaps
+  int vec;                       // runs of features may be moved in 16-byte pieces
+  int smem;
+};
+
+// 16 features n ... of row t, linear.
+template <int ACT>
+__device__ __forceinline__ void finish_features(const Args& a, int vec, int t, int n, const uint32_t (&r)[16]) {
+  if (t >= a.T) return;
+  const size_t at = (size_t)t * a.N + n;
+  if (vec && n + 16 <= a.N) {
+    float v[16];
+    float4 res[4];
+    if (a.residual) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const float4*>(a.residual + at)[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 b = a.bias ? reinterpret_cast<const float4*>(a.bias + n)[j] : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[4 * j] = __uint_as_float(r[4 * j]) + b.x; v[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + b.y;
+      v[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + b.z; v[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + b.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = apply_activation_tc<ACT>(v[j], a.act);
+    if (a.residual) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[4 * j] += res[j].x; v[4 * j + 1] += res[j].y; v[4 * j + 2] += res[j].z; v[4 * j + 3] += res[j].w; }
+    }
+    if (a.out_bf16) {
+      uint32_t p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        p[j] = *reinterpret_cast<const uint32_t*>(&two);
+      }
+      uint4* c = reinterpret_cast<uint4*>((__nv_bfloat16*)a.C + at);
+      c[0] = make_uint4(p[0], p[1], p[2], p[3]);
+      c[1] = make_uint4(p[4], p[5], p[6], p[7]);
+    } else {
+      float4* c = reinterpret_cast<float4*>((float*)a.C + at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if (n + j < a.N) {
+      const float y = apply_activation_tc<ACT>(__uint_as_float(r[j]) + (a.bias ? a.bias[n + j] : 0.f), a.act) + (a.residual ? a.residual[at + j] : 0.f);
+      if (a.out_bf16) ((__nv_bfloat16*)a.C)[at + j] = __float2bfloat16_rn(y);
+      else ((float*)a.C)[at + j] = y;
+    }
+  }
+}
+
+// A block of 32 features of row t, gated: the scale and the codes of one thread.
+template <int ACT>
+__device__ __forceinline__ void finish_block(const Args& a, int t, int n, const uint32_t (&g)[32], const uint32_t (&u)[32]) {
+  if (t >= a.T || n >= a.N) return;
+  float v[32];
+  uint32_t largest = 0u;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    v[j] = apply_activation_tc<ACT>(__uint_as_float(g[j]), a.act) * __uint_as_float(u[j]);
+    largest = max(largest, magnitude_bits(v[j]));
+  }
+  const uint32_t code = mx_scale_code(largest);
+  const float inverse = mx_inverse(code);
+  uint32_t p[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    p[j] = e4m3_pair(v[4 * j] * inverse, v[4 * j + 1] * inverse) | (e4m3_pair(v[4 * j + 2] * inverse, v[4 * j + 3] * inverse) << 16);
+  uint4* c = reinterpret_cast<uint4*>((uint8_t*)a.C + (size_t)t * a.N + n);
+  c[0] = make_uint4(p[0], p[1], p[2], p[3]);
+  c[1] = make_uint4(p[4], p[5], p[6], p[7]);
+  a.out_scales[(size_t)t * a.out_scale_stride + n / MX_BLOCK] = (uint8_t)code;
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
+                    const __grid_constant__ CUtensorMap map_a, const Args args, const ManyShape shape) {
+  constexpr int MATRICES = GATED ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  const int BN = shape.BN, stages = shape.stages;
+  const int weight_bytes = BN * BLOCK_K, tile_bytes = ROWS_BYTES + MATRICES * weight_bytes;
+  const int groups = 1 + MATRICES * shape.w_blocks, quad_bytes = groups * QUAD_BYTES;      // a quad: [group][column block][512]
+  const uint32_t raw = smem_u32(smem_raw), tiles = (raw + 1023u) & ~1023u, ring = tiles + stages * tile_bytes, bars = ring + MANY_QUADS * quad_bytes;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (MANY_MOST_STAGES + s); };
+  auto scales_full = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + q); };
+  auto scales_empty = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + MANY_QUADS + q); };
+  auto sums_full = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + b); };
+  auto sums_empty = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + 2 + b); };
+  const uint32_t tmem_slot = bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + 4);
+
+  const int warp = warp_number(), lane = threadIdx.x & 31;
+  const int num_kb = (args.K + BLOCK_K - 1) / BLOCK_K;
+  const int num_tiles = shape.m_tiles * shape.n_tiles;
+
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w0) : "memory");
+    if (GATED) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w1) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int q = 0; q < MANY_QUADS; ++q) {
+      mbar_init(scales_full(q), 2);
+      mbar_init(scales_empty(q), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(sums_full(b), 1);
+      mbar_init(sums_empty(b), 8);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(*(volatile uint32_t*)(smem_raw + (tmem_slot - raw)));
+  pdl_trigger();                 // after the allocation, see above
+
+  bool ok = true;
+  if (warp == 0) {
+    if (elect_one()) {
+      int issued = 0;
+      pdl_wait();
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        const int t0 = tile % shape.m_tiles * TILE_T, n0 = tile / shape.m_tiles * BN;
+        const uint32_t tx = ROWS_BYTES + MATRICES * weight_bytes / 2;      // codes count as they travel, two to a byte
+        for (int kb = 0; kb < num_kb; ++kb, ++issued) {
+          const int s = issued % stages;
+          if (issued >= stages) ok = mbar_wait(empty_bar(s), ((uint32_t)(issued / stages) & 1u) ^ 1u, args.error, 111);
+          if (!ok) break;
+          mbar_expect_tx(full_bar(s), tx);
+          const uint32_t at = tiles + s * tile_bytes;
+          tma_load_2d(at, &map_a, kb * BLOCK_K, t0, full_bar(s));
+#pragma unroll
+          for (int m = 0; m < MATRICES; ++m) tma_load_3d(at + ROWS_BYTES + m * weight_bytes, m ? &map_w1 : &map_w0, 0, n0, kb, full_bar(s));
+        }
+      }
+      if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued
+        for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(full_bar(i % stages), (uint32_t)(i / stages) & 1u, args.error, 112);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc_mx(TILE_T, BN, MX_E4M3, MX_E2M1);
+      int i = 0, quad = 0, it = 0;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
+        const int buffer = it & 1;
+        const uint32_t sums = tmem + buffer * MATRICES * BN;
+        if (it >= 2) ok = mbar_wait(sums_empty(buffer), ((uint32_t)(it >> 1) & 1u) ^ 1u, args.error, 113);
+        for (int kb = 0; kb < num_kb && ok; ++kb, ++i) {
+          const int s = i % stages, q = quad % MANY_QUADS;
+          if ((kb & 3) == 0) ok = mbar_wait(scales_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 114);
+          ok = ok && mbar_wait(full_bar(s), (uint32_t)(i / stages) & 1u, args.error, 115);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t columns = tmem + 2 * MATRICES * BN + s * 4 * groups;      // a stage's own, as above
+          for (int g = 0; g < groups; ++g) tmem_cp_scales(columns + 4 * g, make_desc_scales(ring + q * quad_bytes + g * QUAD_BYTES + (kb & 3) * SCALE_BYTES));
+          const uint32_t at = tiles + s * tile_bytes;
+          const uint64_t rows = make_desc(at);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int m = 0; m < MATRICES; ++m)
+              umma_mx(sums + m * BN, rows + (uint64_t)(2 * k), make_desc(at + ROWS_BYTES + m * weight_bytes) + (uint64_t)(2 * k), idesc_mx_block(idesc, k),
+                      columns, columns + 4 + 4 * m * shape.w_blocks, (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          umma_commit(empty_bar(s));
+          if ((kb & 3) == 3 || kb == num_kb - 1) {
+            umma_commit(scales_empty(q));
+            ++quad;
+          }
+        }
+        umma_commit(sums_full(buffer));
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    pdl_wait();
+    int quad = 0;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int t = tile % shape.m_tiles * TILE_T + lane;
+      for (int first = 0; first < num_kb && ok; first += 4, ++quad) {
+        uint32_t words[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) words[j][k] = row_scales(args, t + 32 * j, first + k);
+        const int q = quad % MANY_QUADS;
+        if (quad >= MANY_QUADS) ok = mbar_wait(scales_empty(q), ((uint32_t)(quad / MANY_QUADS) & 1u) ^ 1u, args.error, 116);
+        if (!ok) break;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ring + q * quad_bytes + k * SCALE_BYTES + lane * 16), "r"(words[0][k]),
+                       "r"(words[1][k]), "r"(words[2][k]), "r"(words[3][k]) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scales_full(q));
+      }
+    }
+  } else if (warp == 3) {
+    int quad = 0;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int n0 = tile / shape.m_tiles * BN, block0 = n0 / TILE_N, shift = n0 % TILE_N / 32;
+      for (int first = 0; first < num_kb && ok; first += 4, ++quad) {
+        uint4 words[MATRICES][MANY_MOST_BLOCKS][4];      // this lane's of a block: rows lane, lane + 32, ...; a whole 512 bytes to a load
+#pragma unroll
+        for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+          for (int b = 0; b < MANY_MOST_BLOCKS; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bool there = 4 * b < shift + BN / 32 && block0 + b < args.n_blocks && first + k < num_kb;
+              words[m][b][k] = there ? *reinterpret_cast<const uint4*>(args.w_scales[m] + ((size_t)(first + k) * args.n_blocks + block0 + b) * SCALE_BYTES + lane * 16)
+                                     : make_uint4(0u, 0u, 0u, 0u);
+            }
+        const int q = quad % MANY_QUADS;
+        if (quad >= MANY_QUADS) ok = mbar_wait(scales_empty(q), ((uint32_t)(quad / MANY_QUADS) & 1u) ^ 1u, args.error, 118);
+        if (!ok) break;
+#pragma unroll
+        for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+          for (int b = 0; b < MANY_MOST_BLOCKS; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t w[4] = {words[m][b][k].x, words[m][b][k].y, words[m][b][k].z, words[m][b][k].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int column = 4 * b + j - shift;            // 32 features' scales
+                if (column >= 0 && column < 4 * shape.w_blocks)
+                  asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + q * quad_bytes + (1 + m * shape.w_blocks + (column >> 2)) * QUAD_BYTES +
+                                                               k * SCALE_BYTES + lane * 16 + (column & 3) * 4), "r"(w[j]) : "memory");
+              }
+            }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scales_full(q));
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    pdl_wait();
+    with_activation(args.act, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      int it = 0;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
+        const int buffer = it & 1, t = tile % shape.m_tiles * TILE_T + quarter * 32 + lane, n0 = tile / shape.m_tiles * BN;
+        ok = mbar_wait(sums_full(buffer), (uint32_t)(it >> 1) & 1u, args.error, 117);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sums = tmem + ((uint32_t)(quarter * 32) << 16) + buffer * MATRICES * BN;
+        constexpr int RUN = GATED ? 32 : 16;
+#pragma unroll 1
+        for (int c = half * RUN; c < BN && n0 + c < args.N; c += 2 * RUN) {
+          if constexpr (GATED) {
+            uint32_t g[32], u[32];
+            tmem_ld32(sums + c, g);
+            tmem_ld32(sums + BN + c, u);
+            tmem_ld_wait();
+            finish_block<ACT>(args, t, n0 + c, g, u);
+          } else {
+            uint32_t r[16];
+            tmem_ld16(sums + c, r);
+            tmem_ld_wait();
+            finish_features<ACT>(args, shape.vec, t, n0 + c, r);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sums_empty(buffer));
+      }
+    });
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ------------------------------------------------------------------- host --
@@ -333,10 +692,10 @@ int encode_weight(CUtensorMap* map, const void* p, int rows, int K, int box) {
   return 0;
 }
 
-// CTAs along K: as many as keep every multiprocessor's two places filled, with four column blocks for each at least.
-int few_splits(int tiles, int blocks_k, int most) {
+// CTAs along K: as many as fill every multiprocessor's places, with four column blocks for each at least.
+int few_splits(int tiles, int blocks_k, int places, int most) {
   int s = 1;
-  while (2 * s <= most && tiles * 2 * s <= 2 * ayk_sm_count() && blocks_k >= 4 * 2 * s) s *= 2;
+  while (2 * s <= most && tiles * 2 * s <= places * ayk_sm_count() && blocks_k >= 4 * 2 * s) s *= 2;
   return s;
 }
 
@@ -345,10 +704,10 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
   using L = Few<BT, GATED>;
   constexpr int MOST = GATED && BT >= 64 ? 4 : 8;                // splits; what their sums leave of shared memory
   static_assert(L::smem(MOST) <= 232448 && L::smem(1) <= 232448, "shared memory");
-  static_assert(L::USED <= 512 && 8 * (2 * L::STAGES + 2 * QUADS + 2) <= 256 && L::AT_BARS % 16 == 0, "layout");
+  static_assert(L::USED <= 512 && 8 * (2 * L::STAGES + 2 * MANY_QUADS + 2) <= 256 && L::AT_BARS % 16 == 0, "layout");
   const int tiles_n = (args.N + TILE_N - 1) / TILE_N, tiles_t = (args.T + BT - 1) / BT;
   AYK_REQUIRE(tiles_t <= 65535, "%s: too many rows (%d)", name, args.T);
-  const int splits = few_splits(tiles_n * tiles_t, (args.K + BLOCK_K - 1) / BLOCK_K, MOST);
+  const int splits = few_splits(tiles_n * tiles_t, (args.K + BLOCK_K - 1) / BLOCK_K, L::PLACES, MOST);
   static AykPerDevice configured;
   {
     std::lock_guard<std::mutex> lock(g_mutex);
@@ -362,7 +721,7 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles_n, tiles_t, splits);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(L::THREADS);
   cfg.dynamicSmemBytes = L::smem(splits);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -375,6 +734,68 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
   cudaLaunchKernelEx(&cfg, linear4_few_kernel<BT, GATED>, w0, w1, a, args);
   return ayk_check_launch(name);
 }
+
+// Width of a tile by the time of its column blocks (clocks: what the stage's bytes take through shared memory, in and out, at 128
+// a clock) and the waves that the tiles make.
+template <bool GATED>
+ManyShape many_shape(int T, int N, int K, int vec) {
+  constexpr int MATRICES = GATED ? 2 : 1;
+  const int widths[6] = {224, 192, 128, 96, 64, 32};
+  const int sms = ayk_sm_count(), num_kb = (K + BLOCK_K - 1) / BLOCK_K;
+  ManyShape best{};
+  double best_time = 0;
+  for (int i = GATED ? 3 : 0; i < 6; ++i) {
+    ManyShape s{};
+    s.BN = widths[i];
+    s.m_tiles = (T + TILE_T - 1) / TILE_T;
+    s.n_tiles = (N + s.BN - 1) / s.BN;
+    s.w_blocks = (s.BN + TILE_N - 1) / TILE_N;
+    s.vec = vec;
+    const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K, groups = 1 + MATRICES * s.w_blocks;
+    s.smem = 1024 + MANY_QUADS * groups * QUAD_BYTES + 256;
+    s.stages = (232448 - s.smem) / stage;
+    if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * groups);
+    if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;
+    s.smem += s.stages * stage;
+    const long long tiles = (long long)s.m_tiles * s.n_tiles;
+    const double block = (2.0 * ROWS_BYTES + MATRICES * 1.5 * s.BN * BLOCK_K) / 128;
+    const double time = (double)((tiles + sms - 1) / sms) * num_kb * block + 20.0 * MATRICES * s.BN;
+    if (best_time == 0 || time < best_time) {
+      best = s;
+      best_time = time;
+    }
+  }
+  return best;
+}
+
+template <bool GATED>
+int launch_many(const void* codes0, const void* codes1, const void* a, long long a_stride, const Args& args, const char* name, cudaStream_t stream) {
+  const bool vec = args.N % 8 == 0 && (uintptr_t)args.C % 16 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 16 == 0;
+  const ManyShape s = many_shape<GATED>(args.T, args.N, args.K, vec);
+  const long long tiles = (long long)s.m_tiles * s.n_tiles;
+  AYK_REQUIRE(tiles <= 0x7fffffff - 65536, "%s: too many rows (%d) and columns (%d)", name, args.T, args.N);
+  CUtensorMap w0, w1, rows;
+  const int padded = args.n_blocks * TILE_N;
+  if (encode_weight(&w0, codes0, padded, args.K, s.BN) != 0 || encode_weight(&w1, codes1, padded, args.K, s.BN) != 0 ||
+      encode_rows(&rows, a, args.T, args.K, a_stride, TILE_T) != 0)
+    return -1;
+  static AykPerDevice configured;
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    bool& done = configured.here();
+    if (!done) {
+      const cudaError_t err = cudaFuncSetAttribute(linear4_many_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+      if (err != cudaSuccess) return ayk_fail("%s: shared memory: %s", name, cudaGetErrorString(err));
+      done = true;
+    }
+  }
+  const int sms = ayk_sm_count();
+  ayk_launch(linear4_many_kernel<GATED>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(MANY_THREADS),
+             (size_t)s.smem, stream, w0, w1, rows, args, s);
+  return ayk_check_launch(name);
+}
+
+constexpr int FEW_ROWS = 64;
 
 int check(const char* name, const void* a, long long a_stride, const void* a_scales, long long a_scale_stride, long long T, int N, int K, int act) {
   AYK_REQUIRE(N > 0 && K > 0 && K % MX_BLOCK == 0, "%s: a product of %d columns over rows of %d (whole blocks of %d)", name, N, K, MX_BLOCK);
@@ -403,14 +824,14 @@ AYK_EXPORT int ayk_linear4(void* C, const void* a, long long a_stride, const voi
   args.C = C; args.a_scales = (const uint8_t*)a_scales; args.a_scale_stride = a_scale_stride; args.w_scales[0] = (const uint8_t*)scales;
   args.bias = bias; args.residual = residual; args.error = g_error_dev; args.T = (int)T; args.N = N; args.K = K;
   args.n_blocks = (N + TILE_N - 1) / TILE_N; args.act = act; args.out_bf16 = out_dtype == AYK_DTYPE_BF16;
-  const int bt = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  if (T > FEW_ROWS) return launch_many<false>(codes, codes, a, a_stride, args, "ayk_linear4", stream);
+  const int bt = T <= 16 ? 16 : T <= 32 ? 32 : 64;
   CUtensorMap mw, ma;
   if (encode_weight(&mw, codes, args.n_blocks * TILE_N, K, TILE_N) != 0 || encode_rows(&ma, a, T, K, a_stride, bt) != 0) return -1;
   switch (bt) {
     case 16: return launch_few<16, false>(mw, mw, ma, args, "ayk_linear4", stream);
     case 32: return launch_few<32, false>(mw, mw, ma, args, "ayk_linear4", stream);
-    case 64: return launch_few<64, false>(mw, mw, ma, args, "ayk_linear4", stream);
-    default: return launch_few<128, false>(mw, mw, ma, args, "ayk_linear4", stream);
+    default: return launch_few<64, false>(mw, mw, ma, args, "ayk_linear4", stream);
   }
 }
 
@@ -427,6 +848,8 @@ AYK_EXPORT int ayk_gated_linear4(void* out, void* out_scales, long long out_scal
   args.a_scales = (const uint8_t*)a_scales; args.a_scale_stride = a_scale_stride;
   args.w_scales[0] = (const uint8_t*)gate_scales; args.w_scales[1] = (const uint8_t*)up_scales; args.error = g_error_dev;
   args.T = (int)T; args.N = N; args.K = K; args.n_blocks = (N + TILE_N - 1) / TILE_N; args.act = act;
+  AYK_REQUIRE((uintptr_t)out % 16 == 0, "ayk_gated_linear4: codes must lie on 16-byte boundaries");
+  if (T > FEW_ROWS) return launch_many<true>(gate_codes, up_codes, a, a_stride, args, "ayk_gated_linear4", stream);
   const int bt = T <= 16 ? 16 : T <= 32 ? 32 : 64;
   CUtensorMap mg, mu, ma;
   if (encode_weight(&mg, gate_codes, args.n_blocks * TILE_N, K, TILE_N) != 0 || encode_weight(&mu, up_codes, args.n_blocks * TILE_N, K, TILE_N) != 0 ||

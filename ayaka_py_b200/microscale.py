@@ -22,8 +22,8 @@ class FormatError(ValueError):
 
 
 def scale_columns(width: int) -> int:
-    """Bytes from one row's scales to the next row's: the kernels read them in whole 16-byte pieces."""
-    return -(-(width // BLOCK) // 16) * 16
+    """Bytes from one row's scales to the next row's: the kernels read them four at a time."""
+    return (width // BLOCK + 3) & ~3
 
 
 class Rows8:
@@ -51,8 +51,8 @@ class Rows8:
     def empty(cls, rows: int, width: int, device) -> "Rows8":
         """Rows to be written, laid out as the kernels read them."""
         made = cls.__new__(cls)
-        made.codes = torch.empty((rows, width), dtype=torch.float8_e4m3fn, device=device)
-        made.scales = torch.empty((rows, scale_columns(width)), dtype=torch.float8_e8m0fnu, device=device)[:, :width // BLOCK]
+        made.codes = torch.empty_strided((rows, width), (width, 1), dtype=torch.float8_e4m3fn, device=device)      # the quickest of torch's allocations
+        made.scales = torch.empty_strided((rows, width // BLOCK), (scale_columns(width), 1), dtype=torch.float8_e8m0fnu, device=device)
         return made
 
     @property

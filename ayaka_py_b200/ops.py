@@ -26,6 +26,16 @@ ACTIVATIONS = {"none": 0, "gelu_erf": 1, "gelu_tanh": 2, "quick_gelu": 3, "relu2
 _lib = None
 _lock = threading.Lock()
 
+# Entry points whose arguments ctypes converts by their declared types: a call with a dozen arguments takes 3 us less than with
+# an object made for each.
+_P, _L, _I, _F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
+_DECLARED = {
+    "ayk_rows8": (_P, _P, _L, _P, _L, _L, _I, _I, _P),
+    "ayk_rmsnorm_rows8": (_P, _P, _L, _P, _L, _P, _L, _I, _P, _L, _I, _F, _P),
+    "ayk_linear4": (_P, _P, _L, _P, _L, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P),
+    "ayk_gated_linear4": (_P, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _L, _I, _I, _I, _P),
+}
+
 
 class KernelError(RuntimeError):
     """A kernel refused its arguments or its launch failed."""
@@ -40,6 +50,8 @@ def library():
                 path = _build.build()
                 lib = ctypes.CDLL(str(path))
                 lib.ayk_last_error.restype = ctypes.c_char_p
+                for name, types in _DECLARED.items():
+                    getattr(lib, name).argtypes = types
                 _lib = lib
     return _lib
 
@@ -1776,15 +1788,16 @@ def linear(a: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
 
 # --------------------------------------- rows in 8 bits, weights in 4 bits --
 
-def _here(name: str, *tensors: torch.Tensor | None) -> None:
-    """Kernels run on the current device's current stream: tensors of another device are refused."""
+def _here(name: str, *tensors: torch.Tensor | None) -> int:
+    """The current device's current stream, on which the kernel runs: tensors of another device are refused."""
     device = torch._C._cuda_getDevice()
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise KernelError(f"{name}: a tensor on {t.device}, the current device is cuda:{device}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
-def _stride(t: torch.Tensor) -> int:
+def _apart(t: torch.Tensor) -> int:
     """Numbers from a row to the next; of a single row, whose stride says nothing, its width."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -1795,13 +1808,11 @@ def rows8(x: torch.Tensor) -> Rows8:
     lib = _ready()
     if x.dim() != 2 or x.shape[1] < BLOCK or x.shape[1] % BLOCK or x.stride(1) != 1:
         raise KernelError(f"rows8: rows must be [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(x.shape)}")
-    tag = _tag(x.dtype)
-    _here("rows8", x)
-    T, K = x.shape
+    tag, (T, K) = _tag(x.dtype), x.shape
+    stream = _here("rows8", x)
     out = Rows8.empty(T, K, x.device)
     if T:
-        _launch(lib.ayk_rows8(_ptr(out.codes), _ptr(out.scales), ctypes.c_longlong(out.scales.stride(0)), _ptr(x),
-                              ctypes.c_longlong(_stride(x)), ctypes.c_longlong(T), ctypes.c_int(K), ctypes.c_int(tag), _stream()))
+        _launch(lib.ayk_rows8(out.codes.data_ptr(), out.scales.data_ptr(), _apart(out.scales), x.data_ptr(), _apart(x), T, K, tag, stream))
     return out
 
 
@@ -1813,19 +1824,20 @@ def rmsnorm_rows8(x: torch.Tensor, weight: torch.Tensor, eps: float, y: torch.Te
     if x.dim() != 2 or x.dtype != torch.float32 or x.shape[1] < BLOCK or x.shape[1] % BLOCK or x.stride(1) != 1:
         raise KernelError(f"rmsnorm_rows8: the stream must be float32 [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(x.shape)} of {x.dtype}")
     T, K = x.shape
-    if y is not None and (T > 1 and x.stride(0) < K):
-        raise KernelError("rmsnorm_rows8: rows that are written must not overlap")
     if _f32(weight, "weight").numel() != K:
         raise KernelError("rmsnorm_rows8: weight must be float32 of the row width")
-    if y is not None and (y.shape != x.shape or y.stride(1) != 1):
-        raise KernelError("rmsnorm_rows8: y must have the stream's shape and unit column stride")
-    tag = F32 if y is None else _tag(y.dtype)
-    _here("rmsnorm_rows8", x, weight, y)
+    tag, y_at, y_apart = F32, 0, 0
+    if y is not None:
+        if y.shape != x.shape or y.stride(1) != 1:
+            raise KernelError("rmsnorm_rows8: y must have the stream's shape and unit column stride")
+        if T > 1 and x.stride(0) < K:
+            raise KernelError("rmsnorm_rows8: rows that are written must not overlap")
+        tag, y_at, y_apart = _tag(y.dtype), y.data_ptr(), _apart(y)
+    stream = _here("rmsnorm_rows8", x, weight, y)
     out = Rows8.empty(T, K, x.device)
     if T:
-        _launch(lib.ayk_rmsnorm_rows8(_ptr(out.codes), _ptr(out.scales), ctypes.c_longlong(out.scales.stride(0)), _ptr(x),
-                                      ctypes.c_longlong(_stride(x)), _ptr(y), ctypes.c_longlong(0 if y is None else _stride(y)),
-                                      ctypes.c_int(tag), _ptr(weight), ctypes.c_longlong(T), ctypes.c_int(K), ctypes.c_float(eps), _stream()))
+        _launch(lib.ayk_rmsnorm_rows8(out.codes.data_ptr(), out.scales.data_ptr(), _apart(out.scales), x.data_ptr(), _apart(x), y_at, y_apart,
+                                      tag, weight.data_ptr(), T, K, eps, stream))
     return out
 
 
@@ -1834,11 +1846,13 @@ def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: 
     """act(a @ w^T + bias) (+ residual): rows in 8 bits times a weight in 4, products exact, sums, activation (as ``linear``) and
     residual (float32; it may be ``out``) in 32-bit."""
     lib = _ready()
-    T, K = a.codes.shape
+    codes, scales = a.codes, a.scales
+    T, K = codes.shape
     N = w.shape[0]
     if w.shape[1] != K:
         raise KernelError(f"linear4: operands do not fit: rows {(T, K)}, weight {w.shape}")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise KernelError(f"linear4: unknown activation {activation!r}; known: {sorted(ACTIVATIONS)}")
     tag = _tag(out_dtype)
     if out is not None and (tuple(out.shape) != (T, N) or out.dtype != out_dtype or not out.is_contiguous()):
@@ -1847,14 +1861,13 @@ def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: 
         raise KernelError("linear4: one bias per column")
     if residual is not None and tuple(_f32(residual, "residual").shape) != (T, N):
         raise KernelError("linear4: residual must have the output's shape")
-    _here("linear4", a.codes, w.codes, bias, residual, out)
+    stream = _here("linear4", codes, w.codes, bias, residual, out)
     if out is None:
-        out = torch.empty((T, N), dtype=out_dtype, device=a.codes.device)
+        out = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=codes.device)
     if T:
-        _launch(lib.ayk_linear4(_ptr(out), _ptr(a.codes), ctypes.c_longlong(_stride(a.codes)), _ptr(a.scales),
-                                ctypes.c_longlong(_stride(a.scales)), _ptr(w.codes), _ptr(w.scales), _ptr(bias), _ptr(residual),
-                                ctypes.c_longlong(T), ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(ACTIVATIONS[activation]),
-                                ctypes.c_int(tag), _stream()))
+        _launch(lib.ayk_linear4(out.data_ptr(), codes.data_ptr(), _apart(codes), scales.data_ptr(), _apart(scales), w.codes.data_ptr(),
+                                w.scales.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+                                T, N, K, act, tag, stream))
     return out
 
 
@@ -1862,21 +1875,22 @@ def gated_linear4(a: Rows8, gate: Matrix4, up: Matrix4, activation: str = "silu"
     """act(a @ gate^T) * (a @ up^T) in 8 bits: the first half of a gated feed-forward, whose rows the second half's ``linear4``
     reads.  Both products' sums, the activation and their product are 32-bit; the code is the one rounding."""
     lib = _ready()
-    T, K = a.codes.shape
+    codes, scales = a.codes, a.scales
+    T, K = codes.shape
     N = gate.shape[0]
     if gate.shape != up.shape or gate.shape[1] != K:
         raise KernelError(f"gated_linear4: operands do not fit: rows {(T, K)}, weights {gate.shape} and {up.shape}")
     if N % BLOCK:
         raise KernelError(f"gated_linear4: a row of {N} is not whole blocks of {BLOCK}")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise KernelError(f"gated_linear4: unknown activation {activation!r}; known: {sorted(ACTIVATIONS)}")
-    _here("gated_linear4", a.codes, gate.codes, up.codes)
-    out = Rows8.empty(T, N, a.codes.device)
+    stream = _here("gated_linear4", codes, gate.codes, up.codes)
+    out = Rows8.empty(T, N, codes.device)
     if T:
-        _launch(lib.ayk_gated_linear4(_ptr(out.codes), _ptr(out.scales), ctypes.c_longlong(out.scales.stride(0)), _ptr(a.codes),
-                                      ctypes.c_longlong(_stride(a.codes)), _ptr(a.scales), ctypes.c_longlong(_stride(a.scales)),
-                                      _ptr(gate.codes), _ptr(gate.scales), _ptr(up.codes), _ptr(up.scales), ctypes.c_longlong(T),
-                                      ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(ACTIVATIONS[activation]), _stream()))
+        _launch(lib.ayk_gated_linear4(out.codes.data_ptr(), out.scales.data_ptr(), _apart(out.scales), codes.data_ptr(), _apart(codes),
+                                      scales.data_ptr(), _apart(scales), gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
+                                      up.scales.data_ptr(), T, N, K, act, stream))
     return out
 
 
@@ -1983,7 +1997,7 @@ MIXED_DECODE_MIN = 1     # single-token requests in a mixed step from which they
 def tc_error() -> int:
     """0, or the code of the bounded wait that ran out in a tensor-core kernel
     (1-4: matrix product, 11-17: attention, 51-58: latent attention, 61-68: per-head products, 80-91: attention of wide heads,
-    101-106: products of 4-bit weights)."""
+    101-118: products of 4-bit weights)."""
     lib = library()
     return (int(lib.ayk_gemm_tc_error()) or int(lib.ayk_attention_tc_error())
             or int(lib.ayk_gemm_tc_prefill_error()) or int(lib.ayk_latent_tc_error()) or int(lib.ayk_head_tc_error())
