@@ -4,48 +4,186 @@
 //   x += y;  h = x / sqrt(mean(x^2) + eps) * w;  per block of 32 columns: scale 2^e, codes e4m3(h / 2^e)
 //
 // The sum of squares, the norm and the block's scale are 32-bit; the code is the one rounding.
+//
+// Bound by memory: every number is read once and kept in registers between the sum and the codes.  A thread holds runs of eight
+// numbers, four neighbouring threads a block; a row's threads make its sum of squares through shuffles and one exchange.
 #include "microscale.cuh"
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int RUN = 8;
 
-// One block per row; a warp takes 32 columns at a time, a lane one of them.
-template <typename X, typename Y, bool NORM>
-__global__ void __launch_bounds__(THREADS)
-rows8_kernel(uint8_t* __restrict__ out, uint8_t* scales, long long scale_stride, X* x, long long x_stride, const Y* y,
-             long long y_stride, const float* __restrict__ w, int K, float eps) {
-  __shared__ float red[THREADS / 32];
-  pdl_trigger();
-  pdl_wait();
-  X* row = x + (size_t)blockIdx.x * x_stride;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float inv = 1.f;
-  if constexpr (NORM) {
-    float s = 0.f;
-    for (int k = threadIdx.x; k < K; k += THREADS) {
-      float v = to_float<X>(row[k]);
-      if (y) {
-        v += to_float<Y>(y[(size_t)blockIdx.x * y_stride + k]);
-        row[k] = from_float<X>(v);
-      }
-      s = fmaf(v, v, s);
+__device__ __forceinline__ void load_run(const float* p, bool whole, float (&v)[RUN]) {
+  if (whole) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) v[j] = p[j];
+  }
+}
+__device__ __forceinline__ void load_run(const __nv_bfloat16* p, bool whole, float (&v)[RUN]) {
+  if (whole) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) v[j] = __bfloat162float(p[j]);
+  }
+}
+__device__ __forceinline__ void store_run(float* p, bool whole, const float (&v)[RUN]) {
+  if (whole) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) p[j] = v[j];
+  }
+}
+
+// Run i of a row (`there`: it exists) to its codes and, with its three neighbours, its scale.  Whole warps.
+__device__ __forceinline__ void quantise_run(uint8_t* codes, uint8_t* scales, int i, bool there, const float (&v)[RUN]) {
+  uint32_t largest = 0u;
+#pragma unroll
+  for (int j = 0; j < RUN; ++j) largest = max(largest, magnitude_bits(v[j]));
+  largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+  largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+  const uint32_t code = mx_scale_code(largest);
+  const float inverse = mx_inverse(code);
+  if (there) {
+    uint2 p;
+    p.x = e4m3_pair(v[0] * inverse, v[1] * inverse) | (e4m3_pair(v[2] * inverse, v[3] * inverse) << 16);
+    p.y = e4m3_pair(v[4] * inverse, v[5] * inverse) | (e4m3_pair(v[6] * inverse, v[7] * inverse) << 16);
+    *reinterpret_cast<uint2*>(codes + (size_t)RUN * i) = p;
+    if ((i & 3) == 0) scales[i >> 2] = (uint8_t)code;
+  }
+}
+
+// A row's threads are blockDim.x, whole warps; blockDim.y rows to a block (several only of one warp each).  ITEMS runs to a
+// thread, kept in registers; 0: a row too long for that, whose x is read a second time.
+template <typename X, typename Y, bool NORM, int ITEMS>
+__global__ void rows8_kernel(uint8_t* codes, uint8_t* scales, long long scale_stride, const X* x_in, float* x_out, long long x_stride, const Y* y,
+                             long long y_stride, const float* __restrict__ w, long long rows, int K, float eps, int whole) {
+  __shared__ float red[32];
+  if (gridDim.x <= AYK_FEW_BLOCKS) pdl_trigger();
+  const long long r = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const bool mine = r < rows;                  // whole warps: a row has its own
+  const int runs = K / RUN, threads = blockDim.x;
+  const X* row = x_in + (mine ? r : 0) * x_stride;
+  const Y* add = y ? y + (mine ? r : 0) * y_stride : nullptr;
+  codes += (mine ? r : 0) * K;
+  scales += (mine ? r : 0) * scale_stride;
+  pdl_wait();
+
+  // eight numbers of the row, which takes y's on the way
+  auto fetch = [&](int i, float (&v)[RUN]) {
+    load_run(row + RUN * i, whole & 1, v);
+    if (NORM && add) {
+      float u[RUN];
+      load_run(add + RUN * i, whole & 2, u);
+#pragma unroll
+      for (int j = 0; j < RUN; ++j) v[j] += u[j];
+      store_run(x_out + r * x_stride + RUN * i, whole & 1, v);
+    }
+  };
+  auto total = [&](float s) {
     s = warp_sum(s);
-    if (lane == 0) red[warp] = s;
-    __syncthreads();
-    s = 0.f;
-    for (int i = 0; i < THREADS / 32; ++i) s += red[i];
-    inv = 1.0f / sqrtf(s / (float)K + eps);
+    if (threads > 32) {
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+      __syncthreads();
+      s = 0.f;
+      for (int i = 0; i < threads / 32; ++i) s += red[i];
+    }
+    return s;
+  };
+  auto norm_run = [&](int i, float inv, float (&v)[RUN]) {
+    float g[RUN];
+    load_run(w + RUN * i, whole & 4, g);
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) v[j] = v[j] * inv * g[j];
+  };
+
+  if constexpr (ITEMS > 0) {
+    float v[ITEMS][RUN];
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int i = threadIdx.x + k * threads;
+#pragma unroll
+      for (int j = 0; j < RUN; ++j) v[k][j] = 0.f;
+      if (mine && i < runs) fetch(i, v[k]);
+    }
+    float inv = 1.f;
+    if constexpr (NORM) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) s = fmaf(v[k][j], v[k][j], s);
+      inv = 1.0f / sqrtf(total(s) / (float)K + eps);
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int i = threadIdx.x + k * threads;
+      const bool there = mine && i < runs;
+      if (NORM && there) norm_run(i, inv, v[k]);
+      quantise_run(codes, scales, i, there, v[k]);
+    }
+  } else {
+    float inv = 1.f;
+    if constexpr (NORM) {
+      float s = 0.f;
+      for (int i = threadIdx.x; i < runs; i += threads) {
+        float v[RUN];
+        fetch(i, v);
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) s = fmaf(v[j], v[j], s);
+      }
+      inv = 1.0f / sqrtf(total(s) / (float)K + eps);
+    }
+    for (int first = 0; first < runs; first += threads) {
+      const int i = first + threadIdx.x;
+      float v[RUN] = {};
+      if (i < runs) {
+        load_run(row + RUN * i, whole & 1, v);               // this thread's own stores, where the row was changed
+        if constexpr (NORM) norm_run(i, inv, v);
+      }
+      quantise_run(codes, scales, i, i < runs, v);
+    }
   }
-  for (int b = warp; b < K / MX_BLOCK; b += THREADS / 32) {
-    const int k = b * MX_BLOCK + lane;
-    float v = to_float<X>(row[k]);
-    if constexpr (NORM) v *= inv * w[k];
-    const uint32_t code = mx_scale_code(__reduce_max_sync(0xffffffffu, magnitude_bits(v)));
-    out[(size_t)blockIdx.x * K + k] = (uint8_t)e4m3_pair(v * mx_inverse(code), 0.f);
-    if (lane == 0) scales[(size_t)blockIdx.x * scale_stride + b] = (uint8_t)code;
-  }
+}
+
+constexpr int MOST_THREADS = 512, MOST_ITEMS = 4;
+
+template <typename X, typename Y, bool NORM>
+int launch(const char* name, uint8_t* codes, uint8_t* scales, long long scale_stride, const X* x, long long x_stride, const Y* y, long long y_stride,
+           const float* w, long long T, int K, float eps, cudaStream_t stream) {
+  AYK_REQUIRE(K > 0 && K % MX_BLOCK == 0, "%s: a row of %d is not whole blocks of %d", name, K, MX_BLOCK);
+  AYK_REQUIRE(T >= 0 && T <= 0x7fffffff, "%s: too many rows (%lld)", name, T);
+  AYK_REQUIRE((uintptr_t)codes % 16 == 0, "%s: codes must lie on 16-byte boundaries", name);
+  if (T == 0) return 0;
+  auto aligned = [](const void* p, long long stride, size_t size) { return (uintptr_t)p % 16 == 0 && stride * (long long)size % 16 == 0; };
+  const int whole = (aligned(x, x_stride, sizeof(X)) ? 1 : 0) | (aligned(y, y_stride, sizeof(Y)) ? 2 : 0) | (aligned(w, 0, 4) ? 4 : 0);
+  // As few numbers to a thread as rows of MOST_THREADS allow: a row is a chain of loads, a sum and stores, and many rows are under way.
+  const int runs = K / RUN;
+  int items = 1;
+  while (items <= MOST_ITEMS && (runs + items - 1) / items > MOST_THREADS) items *= 2;
+  const int threads = items > MOST_ITEMS ? MOST_THREADS : ((runs + items - 1) / items + 31) / 32 * 32;
+  const dim3 block(threads, threads == 32 ? 4 : 1);
+  const dim3 grid((unsigned)((T + block.y - 1) / block.y));
+  float* x_out = (float*)const_cast<X*>(x);
+#define ROWS8_LAUNCH(ITEMS) \
+  ayk_launch(rows8_kernel<X, Y, NORM, ITEMS>, grid, block, 0, stream, codes, scales, scale_stride, x, x_out, x_stride, y, y_stride, w, T, K, eps, whole)
+  if (items == 1) ROWS8_LAUNCH(1);
+  else if (items == 2) ROWS8_LAUNCH(2);
+  else if (items == 4) ROWS8_LAUNCH(4);
+  else ROWS8_LAUNCH(0);
+#undef ROWS8_LAUNCH
+  return ayk_check_launch(name);
 }
 
 }  // namespace
@@ -53,33 +191,21 @@ rows8_kernel(uint8_t* __restrict__ out, uint8_t* scales, long long scale_stride,
 // codes [T, K] and scales (rows `scale_stride` bytes apart) of x [T, K], rows `x_stride` numbers apart.
 AYK_EXPORT int ayk_rows8(void* codes, void* scales, long long scale_stride, const void* x, long long x_stride, long long T, int K, int dtype,
                          cudaStream_t stream) {
-  AYK_REQUIRE(K > 0 && K % MX_BLOCK == 0, "ayk_rows8: a row of %d is not whole blocks of %d", K, MX_BLOCK);
   AYK_REQUIRE(dtype == AYK_DTYPE_F32 || dtype == AYK_DTYPE_BF16, "ayk_rows8: unknown dtype %d", dtype);
-  AYK_REQUIRE(T >= 0 && T <= 0x7fffffff, "ayk_rows8: too many rows");
-  if (T == 0) return 0;
-  uint8_t *c = (uint8_t*)codes, *s = (uint8_t*)scales;
+  const float* none = nullptr;
   if (dtype == AYK_DTYPE_F32)
-    ayk_launch(rows8_kernel<float, float, false>, dim3((unsigned)T), dim3(THREADS), 0, stream, c, s, scale_stride, (float*)x, x_stride,
-               (const float*)nullptr, 0ll, (const float*)nullptr, K, 0.f);
-  else
-    ayk_launch(rows8_kernel<__nv_bfloat16, float, false>, dim3((unsigned)T), dim3(THREADS), 0, stream, c, s, scale_stride, (__nv_bfloat16*)x,
-               x_stride, (const float*)nullptr, 0ll, (const float*)nullptr, K, 0.f);
-  return ayk_check_launch("ayk_rows8");
+    return launch<float, float, false>("ayk_rows8", (uint8_t*)codes, (uint8_t*)scales, scale_stride, (const float*)x, x_stride, none, 0, none, T, K, 0.f, stream);
+  return launch<__nv_bfloat16, float, false>("ayk_rows8", (uint8_t*)codes, (uint8_t*)scales, scale_stride, (const __nv_bfloat16*)x, x_stride, none, 0, none, T, K,
+                                             0.f, stream);
 }
 
 // x (float32) += y (float32 or bfloat16; null: nothing), and codes and scales of the norm of the new x.
 AYK_EXPORT int ayk_rmsnorm_rows8(void* codes, void* scales, long long scale_stride, void* x, long long x_stride, const void* y, long long y_stride,
                                  int y_dtype, const float* w, long long T, int K, float eps, cudaStream_t stream) {
-  AYK_REQUIRE(K > 0 && K % MX_BLOCK == 0, "ayk_rmsnorm_rows8: a row of %d is not whole blocks of %d", K, MX_BLOCK);
   AYK_REQUIRE(y_dtype == AYK_DTYPE_F32 || y_dtype == AYK_DTYPE_BF16, "ayk_rmsnorm_rows8: unknown dtype %d", y_dtype);
-  AYK_REQUIRE(T >= 0 && T <= 0x7fffffff, "ayk_rmsnorm_rows8: too many rows");
-  if (T == 0) return 0;
-  uint8_t *c = (uint8_t*)codes, *s = (uint8_t*)scales;
   if (y_dtype == AYK_DTYPE_F32)
-    ayk_launch(rows8_kernel<float, float, true>, dim3((unsigned)T), dim3(THREADS), 0, stream, c, s, scale_stride, (float*)x, x_stride,
-               (const float*)y, y_stride, w, K, eps);
-  else
-    ayk_launch(rows8_kernel<float, __nv_bfloat16, true>, dim3((unsigned)T), dim3(THREADS), 0, stream, c, s, scale_stride, (float*)x, x_stride,
-               (const __nv_bfloat16*)y, y_stride, w, K, eps);
-  return ayk_check_launch("ayk_rmsnorm_rows8");
+    return launch<float, float, true>("ayk_rmsnorm_rows8", (uint8_t*)codes, (uint8_t*)scales, scale_stride, (const float*)x, x_stride, (const float*)y, y_stride,
+                                      w, T, K, eps, stream);
+  return launch<float, __nv_bfloat16, true>("ayk_rmsnorm_rows8", (uint8_t*)codes, (uint8_t*)scales, scale_stride, (const float*)x, x_stride,
+                                            (const __nv_bfloat16*)y, y_stride, w, T, K, eps, stream);
 }

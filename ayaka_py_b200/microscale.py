@@ -29,9 +29,9 @@ def scale_columns(width: int) -> int:
 class Rows8:
     """``codes`` [T, K] float8_e4m3fn and ``scales`` [T, K / 32] float8_e8m0fnu: row t is codes[t, k] * scales[t, k // 32].
     Tensors that do not lie as the kernels read them (rows of codes from 16-byte boundaries, rows of scales from 4-byte
-    boundaries, columns side by side) are copied into such."""
+    boundaries, columns side by side) are copied into such.  ``apart``: bytes from a row of codes, and of scales, to the next."""
 
-    __slots__ = ("codes", "scales")
+    __slots__ = ("codes", "scales", "apart")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dim() != 2 or codes.dtype != torch.float8_e4m3fn:
@@ -46,13 +46,15 @@ class Rows8:
         if (K > BLOCK and scales.stride(1) != 1) or (T > 1 and (scales.stride(0) % 4 or scales.stride(0) < K // BLOCK)) or scales.data_ptr() % 4:
             scales = torch.empty((T, scale_columns(K)), dtype=scales.dtype, device=scales.device)[:, :K // BLOCK].copy_(scales)
         self.codes, self.scales = codes, scales
+        self.apart = (codes.stride(0), scales.stride(0)) if T > 1 else (K, scale_columns(K))      # a single row's stride says nothing
 
     @classmethod
     def empty(cls, rows: int, width: int, device) -> "Rows8":
         """Rows to be written, laid out as the kernels read them."""
         made = cls.__new__(cls)
+        made.apart = apart = (width, (width // BLOCK + 3) & ~3)
         made.codes = torch.empty_strided((rows, width), (width, 1), dtype=torch.float8_e4m3fn, device=device)      # the quickest of torch's allocations
-        made.scales = torch.empty_strided((rows, width // BLOCK), (scale_columns(width), 1), dtype=torch.float8_e8m0fnu, device=device)
+        made.scales = torch.empty_strided((rows, width // BLOCK), (apart[1], 1), dtype=torch.float8_e8m0fnu, device=device)
         return made
 
     @property

@@ -1788,31 +1788,26 @@ def linear(a: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
 
 # --------------------------------------- rows in 8 bits, weights in 4 bits --
 
-def _here(name: str, *tensors: torch.Tensor | None) -> int:
-    """The current device's current stream, on which the kernel runs: tensors of another device are refused."""
-    device = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise KernelError(f"{name}: a tensor on {t.device}, the current device is cuda:{device}")
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-def _apart(t: torch.Tensor) -> int:
-    """Numbers from a row to the next; of a single row, whose stride says nothing, its width."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _elsewhere(name: str, device: int, *tensors: torch.Tensor | None) -> KernelError:
+    """Kernels run on the current device's current stream: the first of the tensors that is on another device, as an error."""
+    t = next(t for t in tensors if t is not None and t.get_device() != device)
+    return KernelError(f"{name}: a tensor on {t.device}, the current device is cuda:{device}")
 
 
 def rows8(x: torch.Tensor) -> Rows8:
     """Rows [T, K] of float32 or bfloat16 (columns side by side; they may be columns of a wider matrix) in 8 bits: e4m3 numbers
     with a power of two for every 32 columns (``microscale``)."""
     lib = _ready()
-    if x.dim() != 2 or x.shape[1] < BLOCK or x.shape[1] % BLOCK or x.stride(1) != 1:
-        raise KernelError(f"rows8: rows must be [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(x.shape)}")
-    tag, (T, K) = _tag(x.dtype), x.shape
-    stream = _here("rows8", x)
+    shape, apart = x.shape, x.stride()
+    if len(shape) != 2 or shape[1] < BLOCK or shape[1] % BLOCK or apart[1] != 1:
+        raise KernelError(f"rows8: rows must be [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(shape)}")
+    (T, K), tag, device = shape, _tag(x.dtype), torch._C._cuda_getDevice()
+    if x.get_device() != device:
+        raise _elsewhere("rows8", device, x)
     out = Rows8.empty(T, K, x.device)
     if T:
-        _launch(lib.ayk_rows8(out.codes.data_ptr(), out.scales.data_ptr(), _apart(out.scales), x.data_ptr(), _apart(x), T, K, tag, stream))
+        _launch(lib.ayk_rows8(out.codes.data_ptr(), out.scales.data_ptr(), out.apart[1], x.data_ptr(), apart[0] if T > 1 else K, T, K, tag,
+                              torch._C._cuda_getCurrentRawStream(device)))
     return out
 
 
@@ -1821,23 +1816,26 @@ def rmsnorm_rows8(x: torch.Tensor, weight: torch.Tensor, eps: float, y: torch.Te
     ``y``: a sublayer's result, float32 or bfloat16 (None: x stays as it is).  x and y may be columns of wider matrices, but
     not overlap."""
     lib = _ready()
-    if x.dim() != 2 or x.dtype != torch.float32 or x.shape[1] < BLOCK or x.shape[1] % BLOCK or x.stride(1) != 1:
-        raise KernelError(f"rmsnorm_rows8: the stream must be float32 [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(x.shape)} of {x.dtype}")
-    T, K = x.shape
+    shape, apart = x.shape, x.stride()
+    if len(shape) != 2 or x.dtype != torch.float32 or shape[1] < BLOCK or shape[1] % BLOCK or apart[1] != 1:
+        raise KernelError(f"rmsnorm_rows8: the stream must be float32 [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(shape)} of {x.dtype}")
+    T, K = shape
+    device = torch._C._cuda_getDevice()
     if _f32(weight, "weight").numel() != K:
         raise KernelError("rmsnorm_rows8: weight must be float32 of the row width")
     tag, y_at, y_apart = F32, 0, 0
     if y is not None:
-        if y.shape != x.shape or y.stride(1) != 1:
+        if y.shape != shape or y.stride(1) != 1:
             raise KernelError("rmsnorm_rows8: y must have the stream's shape and unit column stride")
-        if T > 1 and x.stride(0) < K:
+        if T > 1 and apart[0] < K:
             raise KernelError("rmsnorm_rows8: rows that are written must not overlap")
-        tag, y_at, y_apart = _tag(y.dtype), y.data_ptr(), _apart(y)
-    stream = _here("rmsnorm_rows8", x, weight, y)
+        tag, y_at, y_apart = _tag(y.dtype), y.data_ptr(), y.stride(0) if T > 1 else K
+    if x.get_device() != device or weight.get_device() != device or (y is not None and y.get_device() != device):
+        raise _elsewhere("rmsnorm_rows8", device, x, weight, y)
     out = Rows8.empty(T, K, x.device)
     if T:
-        _launch(lib.ayk_rmsnorm_rows8(out.codes.data_ptr(), out.scales.data_ptr(), _apart(out.scales), x.data_ptr(), _apart(x), y_at, y_apart,
-                                      tag, weight.data_ptr(), T, K, eps, stream))
+        _launch(lib.ayk_rmsnorm_rows8(out.codes.data_ptr(), out.scales.data_ptr(), out.apart[1], x.data_ptr(), apart[0] if T > 1 else K, y_at, y_apart,
+                                      tag, weight.data_ptr(), T, K, eps, torch._C._cuda_getCurrentRawStream(device)))
     return out
 
 
@@ -1846,28 +1844,33 @@ def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: 
     """act(a @ w^T + bias) (+ residual): rows in 8 bits times a weight in 4, products exact, sums, activation (as ``linear``) and
     residual (float32; it may be ``out``) in 32-bit."""
     lib = _ready()
-    codes, scales = a.codes, a.scales
-    T, K = codes.shape
-    N = w.shape[0]
-    if w.shape[1] != K:
+    codes = a.codes
+    (T, K), (N, width), device = codes.shape, w.shape, torch._C._cuda_getDevice()
+    if width != K:
         raise KernelError(f"linear4: operands do not fit: rows {(T, K)}, weight {w.shape}")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise KernelError(f"linear4: unknown activation {activation!r}; known: {sorted(ACTIVATIONS)}")
-    tag = _tag(out_dtype)
+    tag, bias_at, residual_at = _tag(out_dtype), 0, 0
+    if bias is not None:
+        if _f32(bias, "bias").numel() != N:
+            raise KernelError("linear4: one bias per column")
+        bias_at = bias.data_ptr()
+    if residual is not None:
+        if tuple(_f32(residual, "residual").shape) != (T, N):
+            raise KernelError("linear4: residual must have the output's shape")
+        residual_at = residual.data_ptr()
     if out is not None and (tuple(out.shape) != (T, N) or out.dtype != out_dtype or not out.is_contiguous()):
         raise KernelError("linear4: out must be a contiguous [T, N] tensor of the output dtype")
-    if bias is not None and _f32(bias, "bias").numel() != N:
-        raise KernelError("linear4: one bias per column")
-    if residual is not None and tuple(_f32(residual, "residual").shape) != (T, N):
-        raise KernelError("linear4: residual must have the output's shape")
-    stream = _here("linear4", codes, w.codes, bias, residual, out)
+    if (codes.get_device() != device or w.codes.get_device() != device or (bias is not None and bias.get_device() != device)
+            or (residual is not None and residual.get_device() != device) or (out is not None and out.get_device() != device)):
+        raise _elsewhere("linear4", device, codes, w.codes, bias, residual, out)
     if out is None:
         out = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=codes.device)
     if T:
-        _launch(lib.ayk_linear4(out.data_ptr(), codes.data_ptr(), _apart(codes), scales.data_ptr(), _apart(scales), w.codes.data_ptr(),
-                                w.scales.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
-                                T, N, K, act, tag, stream))
+        apart = a.apart
+        _launch(lib.ayk_linear4(out.data_ptr(), codes.data_ptr(), apart[0], a.scales.data_ptr(), apart[1], w.codes.data_ptr(), w.scales.data_ptr(),
+                                bias_at, residual_at, T, N, K, act, tag, torch._C._cuda_getCurrentRawStream(device)))
     return out
 
 
@@ -1875,22 +1878,23 @@ def gated_linear4(a: Rows8, gate: Matrix4, up: Matrix4, activation: str = "silu"
     """act(a @ gate^T) * (a @ up^T) in 8 bits: the first half of a gated feed-forward, whose rows the second half's ``linear4``
     reads.  Both products' sums, the activation and their product are 32-bit; the code is the one rounding."""
     lib = _ready()
-    codes, scales = a.codes, a.scales
-    T, K = codes.shape
-    N = gate.shape[0]
-    if gate.shape != up.shape or gate.shape[1] != K:
+    codes = a.codes
+    (T, K), (N, width), device = codes.shape, gate.shape, torch._C._cuda_getDevice()
+    if width != K or up.shape != gate.shape:
         raise KernelError(f"gated_linear4: operands do not fit: rows {(T, K)}, weights {gate.shape} and {up.shape}")
     if N % BLOCK:
         raise KernelError(f"gated_linear4: a row of {N} is not whole blocks of {BLOCK}")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise KernelError(f"gated_linear4: unknown activation {activation!r}; known: {sorted(ACTIVATIONS)}")
-    stream = _here("gated_linear4", codes, gate.codes, up.codes)
+    if codes.get_device() != device or gate.codes.get_device() != device or up.codes.get_device() != device:
+        raise _elsewhere("gated_linear4", device, codes, gate.codes, up.codes)
     out = Rows8.empty(T, N, codes.device)
     if T:
-        _launch(lib.ayk_gated_linear4(out.codes.data_ptr(), out.scales.data_ptr(), _apart(out.scales), codes.data_ptr(), _apart(codes),
-                                      scales.data_ptr(), _apart(scales), gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
-                                      up.scales.data_ptr(), T, N, K, act, stream))
+        apart = a.apart
+        _launch(lib.ayk_gated_linear4(out.codes.data_ptr(), out.scales.data_ptr(), out.apart[1], codes.data_ptr(), apart[0], a.scales.data_ptr(), apart[1],
+                                      gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(), T, N, K, act,
+                                      torch._C._cuda_getCurrentRawStream(device)))
     return out
 
 
