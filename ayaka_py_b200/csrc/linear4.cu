@@ -7,7 +7,7 @@
 // Weights lie in column blocks of 128 (64 bytes of codes a row), their scales beside them as the tensor cores take them.  The
 // copy engine spreads sixteen codes over sixteen bytes on their way into shared memory.
 //
-// Every wait is bounded; one that runs out records a code (101 ... 118) in an error word and the CTA winds down.
+// Every wait is bounded; one that runs out records a code (101 ... 119) in an error word and the CTA winds down.
 #include <cuda.h>
 
 #include <mutex>
@@ -340,19 +340,24 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
 // gated product BN of each matrix), two accumulators in tensor memory so that a tile's epilogue runs under the next one's main
 // loop.  An epilogue thread owns a row and stores runs of features.
 //
-// Warp 0: copies; warp 1: MMA issue, tensor memory; warp 2: the rows' scales; warp 3: the weights', which it shifts so that a tile's
-// first feature has the first column (the MMA wants its scales from a whole group of four columns on, and a tile may start at any
-// 32 features); warps 4 ... 11: epilogue, two to a quarter of the rows, each with every other run of features.
+// Scales travel for four column blocks (a quad) at a time, as they lie in memory, and are put in order in shared
+// memory: warp 2 turns the rows', of which 16 bytes come for each row; warp 3 shifts the weights' so that a tile's first feature has
+// the first column (the MMA takes its scales from a whole group of four columns on, and a tile may start at any 32 features).
+// Loaded by those warps themselves, a quad after the other, they set the pace: 0.58 us a column block against 0.3.
+//
+// Warp 0: the operands' copies; warp 1: MMA issue, tensor memory; warps 2, 3: scales; warps 4 ... 11: epilogue, two to a quarter of
+// the rows, each with every other run of features; warp 12: the scales' copies.
 constexpr int TILE_T = 128;
-constexpr int MANY_THREADS = 384;
+constexpr int MANY_THREADS = 416;
 constexpr int ROWS_BYTES = TILE_T * BLOCK_K;
 constexpr int MANY_MOST_STAGES = 8;
-constexpr int MANY_QUADS = 3;                   // scales come for four column blocks at a time, into a ring of three such
+constexpr int MANY_QUADS = 2;                   // places of the two rings, of scales as they come and in order
 constexpr int MANY_MOST_BLOCKS = 3;             // of 128 features' scales that a tile of 224 touches
 
 struct ManyShape {
   int BN, stages, m_tiles, n_tiles;
   int w_blocks;                  // groups of 128 features in a tile, the last one not full perhaps
+  int w_touched;                 // aligned groups of 128 features that a tile touches at most
   int vec;                       // runs of features may be moved in 16-byte pieces
   int smem;
 };
@@ -431,23 +436,34 @@ __device__ __forceinline__ void finish_block(const Args& a, int t, int n, const 
   a.out_scales[(size_t)t * a.out_scale_stride + n / MX_BLOCK] = (uint8_t)code;
 }
 
+__device__ __forceinline__ void lds_v4(uint32_t at, uint32_t* w) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void sts_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 template <bool GATED>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
-linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
-                    const __grid_constant__ CUtensorMap map_a, const Args args, const ManyShape shape) {
+linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1, const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_s, const Args args, const ManyShape shape) {
   constexpr int MATRICES = GATED ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   const int BN = shape.BN, stages = shape.stages;
   const int weight_bytes = BN * BLOCK_K, tile_bytes = ROWS_BYTES + MATRICES * weight_bytes;
   const int groups = 1 + MATRICES * shape.w_blocks, quad_bytes = groups * QUAD_BYTES;      // a quad: [group][column block][512]
-  const uint32_t raw = smem_u32(smem_raw), tiles = (raw + 1023u) & ~1023u, ring = tiles + stages * tile_bytes, bars = ring + MANY_QUADS * quad_bytes;
+  const int come_bytes = (1 + MATRICES * shape.w_touched) * QUAD_BYTES;                    // as they come: rows [128][16], features [matrix][group][column block][512]
+  const uint32_t raw = smem_u32(smem_raw), tiles = (raw + 1023u) & ~1023u, ring = tiles + stages * tile_bytes;
+  const uint32_t come = ring + MANY_QUADS * quad_bytes, bars = come + MANY_QUADS * come_bytes;
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (MANY_MOST_STAGES + s); };
   auto scales_full = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + q); };
   auto scales_empty = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + MANY_QUADS + q); };
   auto sums_full = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + b); };
   auto sums_empty = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + 2 + b); };
-  const uint32_t tmem_slot = bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + 4);
+  auto come_full = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + 4 + q); };
+  auto come_empty = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 3 * MANY_QUADS + 4 + q); };
+  const uint32_t tmem_slot = bars + 8u * (2 * MANY_MOST_STAGES + 4 * MANY_QUADS + 4);
 
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int num_kb = (args.K + BLOCK_K - 1) / BLOCK_K;
@@ -464,6 +480,8 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     for (int q = 0; q < MANY_QUADS; ++q) {
       mbar_init(scales_full(q), 2);
       mbar_init(scales_empty(q), 1);
+      mbar_init(come_full(q), 1);
+      mbar_init(come_empty(q), 2);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(sums_full(b), 1);
@@ -485,20 +503,24 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   bool ok = true;
   if (warp == 0) {
     if (elect_one()) {
-      int issued = 0;
       pdl_wait();
+      const uint32_t tx = ROWS_BYTES + MATRICES * weight_bytes / 2;        // codes count as they travel, two to a byte
+      const uint32_t bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0);
+      uint32_t bar = full_bar(0), at = tiles, parity = 1;                  // a barrier's first wait by the opposite parity returns at once
+      int issued = 0;
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
         const int t0 = tile % shape.m_tiles * TILE_T, n0 = tile / shape.m_tiles * BN;
-        const uint32_t tx = ROWS_BYTES + MATRICES * weight_bytes / 2;      // codes count as they travel, two to a byte
-        for (int kb = 0; kb < num_kb; ++kb, ++issued) {
-          const int s = issued % stages;
-          if (issued >= stages) ok = mbar_wait(empty_bar(s), ((uint32_t)(issued / stages) & 1u) ^ 1u, args.error, 111);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          ok = mbar_wait_short(bar + to_empty, parity, args.error, 111);
           if (!ok) break;
-          mbar_expect_tx(full_bar(s), tx);
-          const uint32_t at = tiles + s * tile_bytes;
-          tma_load_2d(at, &map_a, kb * BLOCK_K, t0, full_bar(s));
-#pragma unroll
-          for (int m = 0; m < MATRICES; ++m) tma_load_3d(at + ROWS_BYTES + m * weight_bytes, m ? &map_w1 : &map_w0, 0, n0, kb, full_bar(s));
+          mbar_expect_tx(bar, tx);
+          tma_load_2d(at, &map_a, kb * BLOCK_K, t0, bar);
+          tma_load_3d(at + ROWS_BYTES, &map_w0, 0, n0, kb, bar);
+          if (GATED) tma_load_3d(at + ROWS_BYTES + weight_bytes, &map_w1, 0, n0, kb, bar);
+          ++issued;
+          bar += 8u;
+          at += tile_bytes;
+          if (bar == bars_end) { bar = full_bar(0); at = tiles; parity ^= 1u; }
         }
       }
       if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued
@@ -509,98 +531,113 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = make_idesc_mx(TILE_T, BN, MX_E4M3, MX_E2M1);
-      int i = 0, quad = 0, it = 0;
+      const uint32_t bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0), all_sums = 2 * MATRICES * BN;
+      const uint64_t rows0 = make_desc(tiles), weights0 = make_desc(tiles + ROWS_BYTES), scales0 = make_desc_scales(ring);
+      uint32_t bar = full_bar(0), at = 0, parity = 0, columns = tmem + all_sums;      // this stage's: barrier, 16-byte units from the first on, scales
+      uint32_t q = 0, quad_at = 0, quad_parity = 0;
+      int it = 0;
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
-        const int buffer = it & 1;
-        const uint32_t sums = tmem + buffer * MATRICES * BN;
-        if (it >= 2) ok = mbar_wait(sums_empty(buffer), ((uint32_t)(it >> 1) & 1u) ^ 1u, args.error, 113);
-        for (int kb = 0; kb < num_kb && ok; ++kb, ++i) {
-          const int s = i % stages, q = quad % MANY_QUADS;
-          if ((kb & 3) == 0) ok = mbar_wait(scales_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 114);
-          ok = ok && mbar_wait(full_bar(s), (uint32_t)(i / stages) & 1u, args.error, 115);
+        const uint32_t buffer = it & 1, sums = tmem + buffer * MATRICES * BN;
+        if (it >= 2) ok = mbar_wait_short(sums_empty(buffer), ((uint32_t)(it >> 1) & 1u) ^ 1u, args.error, 113);
+        for (int kb = 0; kb < num_kb && ok; ++kb) {
+          if ((kb & 3) == 0) ok = mbar_wait_short(scales_full(q), quad_parity, args.error, 114);
+          ok = ok && mbar_wait_short(bar, parity, args.error, 115);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t columns = tmem + 2 * MATRICES * BN + s * 4 * groups;      // a stage's own, as above
-          for (int g = 0; g < groups; ++g) tmem_cp_scales(columns + 4 * g, make_desc_scales(ring + q * quad_bytes + g * QUAD_BYTES + (kb & 3) * SCALE_BYTES));
-          const uint32_t at = tiles + s * tile_bytes;
-          const uint64_t rows = make_desc(at);
+          const uint64_t scales = scales0 + quad_at + (uint64_t)((kb & 3) * (SCALE_BYTES >> 4));
+#pragma unroll 1
+          for (int g = 0; g < groups; ++g) tmem_cp_scales(columns + 4 * g, scales + (uint64_t)(g * (QUAD_BYTES >> 4)));      // a stage's own columns, as above
+          const uint64_t rows = rows0 + at, weights = weights0 + at;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
 #pragma unroll
             for (int m = 0; m < MATRICES; ++m)
-              umma_mx(sums + m * BN, rows + (uint64_t)(2 * k), make_desc(at + ROWS_BYTES + m * weight_bytes) + (uint64_t)(2 * k), idesc_mx_block(idesc, k),
-                      columns, columns + 4 + 4 * m * shape.w_blocks, (kb > 0 || k > 0) ? 1u : 0u);
+              umma_mx(sums + m * BN, rows + (uint64_t)(2 * k), weights + (uint64_t)(m * (weight_bytes >> 4) + 2 * k), idesc_mx_block(idesc, k), columns,
+                      columns + 4 + 4 * m * shape.w_blocks, (kb > 0 || k > 0) ? 1u : 0u);
           }
-          umma_commit(empty_bar(s));
+          umma_commit(bar + to_empty);
+          bar += 8u;
+          at += tile_bytes >> 4;
+          columns += 4 * groups;
+          if (bar == bars_end) { bar = full_bar(0); at = 0; columns = tmem + all_sums; parity ^= 1u; }
           if ((kb & 3) == 3 || kb == num_kb - 1) {
             umma_commit(scales_empty(q));
-            ++quad;
+            quad_at += quad_bytes >> 4;
+            if (++q == MANY_QUADS) { q = 0; quad_at = 0; quad_parity ^= 1u; }
           }
         }
         umma_commit(sums_full(buffer));
       }
     }
     __syncwarp();
-  } else if (warp == 2) {
-    pdl_wait();
-    int quad = 0;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      const int t = tile % shape.m_tiles * TILE_T + lane;
-      for (int first = 0; first < num_kb && ok; first += 4, ++quad) {
-        uint32_t words[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) words[j][k] = row_scales(args, t + 32 * j, first + k);
-        const int q = quad % MANY_QUADS;
-        if (quad >= MANY_QUADS) ok = mbar_wait(scales_empty(q), ((uint32_t)(quad / MANY_QUADS) & 1u) ^ 1u, args.error, 116);
-        if (!ok) break;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ring + q * quad_bytes + k * SCALE_BYTES + lane * 16), "r"(words[0][k]),
-                       "r"(words[1][k]), "r"(words[2][k]), "r"(words[3][k]) : "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(scales_full(q));
+  } else if (warp == 12) {
+    if (elect_one()) {
+      int quads = 0;
+      pdl_wait();
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        const int t0 = tile % shape.m_tiles * TILE_T, n0 = tile / shape.m_tiles * BN, block0 = n0 / TILE_N;
+        const int blocks = min((n0 % TILE_N + BN + TILE_N - 1) / TILE_N, args.n_blocks - block0);
+        for (int first = 0; first < num_kb; first += 4, ++quads) {
+          const int q = quads % MANY_QUADS, kbs = min(4, num_kb - first);
+          if (quads >= MANY_QUADS) ok = mbar_wait_short(come_empty(q), ((uint32_t)(quads / MANY_QUADS) & 1u) ^ 1u, args.error, 116);
+          if (!ok) break;
+          mbar_expect_tx(come_full(q), QUAD_BYTES + MATRICES * kbs * blocks * SCALE_BYTES);
+          tma_load_2d(come + q * come_bytes, &map_s, 4 * first, t0, come_full(q));
+          for (int m = 0; m < MATRICES; ++m)
+            for (int k = 0; k < kbs; ++k)      // [matrix][column block][group]: a column block's groups lie side by side in memory too
+              bulk_load(come + q * come_bytes + QUAD_BYTES + (m * 4 + k) * shape.w_touched * SCALE_BYTES,
+                        args.w_scales[m] + ((size_t)(first + k) * args.n_blocks + block0) * SCALE_BYTES, blocks * SCALE_BYTES, come_full(q));
+        }
+      }
+      if (!ok) {
+        for (int i = max(0, quads - MANY_QUADS); i < quads; ++i) mbar_wait(come_full(i % MANY_QUADS), (uint32_t)(i / MANY_QUADS) & 1u, args.error, 112);
       }
     }
-  } else if (warp == 3) {
+    __syncwarp();
+  } else if (warp < 4) {
     int quad = 0;
     for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      const int n0 = tile / shape.m_tiles * BN, block0 = n0 / TILE_N, shift = n0 % TILE_N / 32;
+      const int shift = tile / shape.m_tiles * BN % TILE_N / 32;
       for (int first = 0; first < num_kb && ok; first += 4, ++quad) {
-        uint4 words[MATRICES][MANY_MOST_BLOCKS][4];      // this lane's of a block: rows lane, lane + 32, ...; a whole 512 bytes to a load
-#pragma unroll
-        for (int m = 0; m < MATRICES; ++m)
-#pragma unroll
-          for (int b = 0; b < MANY_MOST_BLOCKS; ++b)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const bool there = 4 * b < shift + BN / 32 && block0 + b < args.n_blocks && first + k < num_kb;
-              words[m][b][k] = there ? *reinterpret_cast<const uint4*>(args.w_scales[m] + ((size_t)(first + k) * args.n_blocks + block0 + b) * SCALE_BYTES + lane * 16)
-                                     : make_uint4(0u, 0u, 0u, 0u);
-            }
         const int q = quad % MANY_QUADS;
-        if (quad >= MANY_QUADS) ok = mbar_wait(scales_empty(q), ((uint32_t)(quad / MANY_QUADS) & 1u) ^ 1u, args.error, 118);
+        const uint32_t from = come + q * come_bytes + lane * 16, to = ring + q * quad_bytes + lane * 16;
+        ok = mbar_wait(come_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 118);
+        if (ok && quad >= MANY_QUADS) ok = mbar_wait(scales_empty(q), ((uint32_t)(quad / MANY_QUADS) & 1u) ^ 1u, args.error, 119);
         if (!ok) break;
+        if (warp == 2) {                     // rows lane, lane + 32, ...: 16 bytes are a row's four column blocks
+          uint32_t w[4][4];
 #pragma unroll
-        for (int m = 0; m < MATRICES; ++m)
+          for (int j = 0; j < 4; ++j) lds_v4(from + j * 512, w[j]);
 #pragma unroll
-          for (int b = 0; b < MANY_MOST_BLOCKS; ++b)
-#pragma unroll
+          for (int k = 0; k < 4; ++k) sts_v4(to + k * SCALE_BYTES, w[0][k], w[1][k], w[2][k], w[3][k]);
+        } else {
+#pragma unroll 1
+          for (int m = 0; m < MATRICES; ++m)
+#pragma unroll 1
             for (int k = 0; k < 4; ++k) {
-              const uint32_t w[4] = {words[m][b][k].x, words[m][b][k].y, words[m][b][k].z, words[m][b][k].w};
+              uint32_t w[4 * MANY_MOST_BLOCKS + 4];                  // this lane's columns of the groups, in a row
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int column = 4 * b + j - shift;            // 32 features' scales
-                if (column >= 0 && column < 4 * shape.w_blocks)
-                  asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + q * quad_bytes + (1 + m * shape.w_blocks + (column >> 2)) * QUAD_BYTES +
-                                                               k * SCALE_BYTES + lane * 16 + (column & 3) * 4), "r"(w[j]) : "memory");
-              }
+              for (int b = 0; b < MANY_MOST_BLOCKS; ++b)
+                if (b < shape.w_touched) lds_v4(from + QUAD_BYTES + ((m * 4 + k) * shape.w_touched + b) * SCALE_BYTES, w + 4 * b);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[4 * MANY_MOST_BLOCKS + j] = 0u;
+              if (shift & 1)
+#pragma unroll
+                for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 1];
+              if (shift & 2)
+#pragma unroll
+                for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 2];
+#pragma unroll
+              for (int b = 0; b < MANY_MOST_BLOCKS - 1; ++b)
+                if (b < shape.w_blocks) sts_v4(to + (1 + m * shape.w_blocks + b) * QUAD_BYTES + k * SCALE_BYTES, w[4 * b], w[4 * b + 1], w[4 * b + 2], w[4 * b + 3]);
             }
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(scales_full(q));
+        if (lane == 0) {
+          mbar_arrive(scales_full(q));
+          mbar_arrive(come_empty(q));
+        }
       }
     }
   } else {
@@ -680,6 +717,15 @@ int encode_rows(CUtensorMap* map, const void* p, long long T, int K, long long s
   if (r != CUDA_SUCCESS) return ayk_fail("ayk_linear4: cuTensorMapEncodeTiled of the rows failed with %d", (int)r);
   return 0;
 }
+// The rows' scales, rows `stride` bytes apart: boxes of 16 bytes (four column blocks) and 128 rows.
+int encode_scales(CUtensorMap* map, const void* p, long long T, int K, long long stride) {
+  cuuint64_t dims[2] = {(cuuint64_t)(K / MX_BLOCK), (cuuint64_t)T}, strides[1] = {(cuuint64_t)stride};
+  cuuint32_t boxes[2] = {16, TILE_T}, step[2] = {1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return ayk_fail("ayk_linear4: cuTensorMapEncodeTiled of the rows' scales failed with %d", (int)r);
+  return 0;
+}
 // A weight's codes [K / 128][rows][128]: boxes of `box` rows, spread to a byte each.
 int encode_weight(CUtensorMap* map, const void* p, int rows, int K, int box) {
   cuuint64_t dims[3] = {BLOCK_K, (cuuint64_t)rows, (cuuint64_t)((K + BLOCK_K - 1) / BLOCK_K)};
@@ -750,9 +796,10 @@ ManyShape many_shape(int T, int N, int K, int vec) {
     s.m_tiles = (T + TILE_T - 1) / TILE_T;
     s.n_tiles = (N + s.BN - 1) / s.BN;
     s.w_blocks = (s.BN + TILE_N - 1) / TILE_N;
+    s.w_touched = ((TILE_N % s.BN == 0 ? 0 : s.BN == 192 ? 64 : 96) + s.BN + TILE_N - 1) / TILE_N;      // a tile starts so far behind a group at most
     s.vec = vec;
     const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K, groups = 1 + MATRICES * s.w_blocks;
-    s.smem = 1024 + MANY_QUADS * groups * QUAD_BYTES + 256;
+    s.smem = 1024 + MANY_QUADS * (groups + 1 + MATRICES * s.w_touched) * QUAD_BYTES + 256;
     s.stages = (232448 - s.smem) / stage;
     if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * groups);
     if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;
@@ -774,10 +821,10 @@ int launch_many(const void* codes0, const void* codes1, const void* a, long long
   const ManyShape s = many_shape<GATED>(args.T, args.N, args.K, vec);
   const long long tiles = (long long)s.m_tiles * s.n_tiles;
   AYK_REQUIRE(tiles <= 0x7fffffff - 65536, "%s: too many rows (%d) and columns (%d)", name, args.T, args.N);
-  CUtensorMap w0, w1, rows;
+  CUtensorMap w0, w1, rows, row_scales;
   const int padded = args.n_blocks * TILE_N;
   if (encode_weight(&w0, codes0, padded, args.K, s.BN) != 0 || encode_weight(&w1, codes1, padded, args.K, s.BN) != 0 ||
-      encode_rows(&rows, a, args.T, args.K, a_stride, TILE_T) != 0)
+      encode_rows(&rows, a, args.T, args.K, a_stride, TILE_T) != 0 || encode_scales(&row_scales, args.a_scales, args.T, args.K, args.a_scale_stride) != 0)
     return -1;
   static AykPerDevice configured;
   {
@@ -791,7 +838,7 @@ int launch_many(const void* codes0, const void* codes1, const void* a, long long
   }
   const int sms = ayk_sm_count();
   ayk_launch(linear4_many_kernel<GATED>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(MANY_THREADS),
-             (size_t)s.smem, stream, w0, w1, rows, args, s);
+             (size_t)s.smem, stream, w0, w1, rows, row_scales, args, s);
   return ayk_check_launch(name);
 }
 
@@ -802,7 +849,7 @@ int check(const char* name, const void* a, long long a_stride, const void* a_sca
   AYK_REQUIRE(T >= 0 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256, "%s: too many rows (%lld) or columns (%d)", name, T, N);
   AYK_REQUIRE(act >= AYK_ACT_NONE && act <= AYK_ACT_SILU, "%s: unknown activation %d", name, act);
   AYK_REQUIRE((uintptr_t)a % 16 == 0 && a_stride % 16 == 0 && a_stride >= K, "%s: rows of codes must lie on 16-byte boundaries", name);
-  AYK_REQUIRE((uintptr_t)a_scales % 4 == 0 && (T <= 1 || a_scale_stride % 4 == 0), "%s: rows of scales must lie on 4-byte boundaries", name);
+  AYK_REQUIRE((uintptr_t)a_scales % 16 == 0 && a_scale_stride % 16 == 0 && a_scale_stride >= K / MX_BLOCK, "%s: rows of scales must lie on 16-byte boundaries", name);
   return 0;
 }
 

@@ -22,13 +22,13 @@ class FormatError(ValueError):
 
 
 def scale_columns(width: int) -> int:
-    """Bytes from one row's scales to the next row's: the kernels read them four at a time."""
-    return (width // BLOCK + 3) & ~3
+    """Bytes from one row's scales to the next row's: the kernels read them in whole 16-byte pieces."""
+    return (width // BLOCK + 15) & ~15
 
 
 class Rows8:
     """``codes`` [T, K] float8_e4m3fn and ``scales`` [T, K / 32] float8_e8m0fnu: row t is codes[t, k] * scales[t, k // 32].
-    Tensors that do not lie as the kernels read them (rows of codes from 16-byte boundaries, rows of scales from 4-byte
+    Tensors that do not lie as the kernels read them (rows of codes and of scales from 16-byte
     boundaries, columns side by side) are copied into such.  ``apart``: bytes from a row of codes, and of scales, to the next."""
 
     __slots__ = ("codes", "scales", "apart")
@@ -43,7 +43,7 @@ class Rows8:
             raise FormatError(f"scales must be {(T, K // BLOCK)} of float8_e8m0fnu beside the codes, got {tuple(scales.shape)} of {scales.dtype}")
         if codes.stride(1) != 1 or (T > 1 and (codes.stride(0) % 16 or codes.stride(0) < K)) or codes.data_ptr() % 16:
             codes = torch.empty((T, K), dtype=codes.dtype, device=codes.device).copy_(codes)
-        if (K > BLOCK and scales.stride(1) != 1) or (T > 1 and (scales.stride(0) % 4 or scales.stride(0) < K // BLOCK)) or scales.data_ptr() % 4:
+        if (K > BLOCK and scales.stride(1) != 1) or (T > 1 and (scales.stride(0) % 16 or scales.stride(0) < K // BLOCK)) or scales.data_ptr() % 16:
             scales = torch.empty((T, scale_columns(K)), dtype=scales.dtype, device=scales.device)[:, :K // BLOCK].copy_(scales)
         self.codes, self.scales = codes, scales
         self.apart = (codes.stride(0), scales.stride(0)) if T > 1 else (K, scale_columns(K))      # a single row's stride says nothing
@@ -52,7 +52,7 @@ class Rows8:
     def empty(cls, rows: int, width: int, device) -> "Rows8":
         """Rows to be written, laid out as the kernels read them."""
         made = cls.__new__(cls)
-        made.apart = apart = (width, (width // BLOCK + 3) & ~3)
+        made.apart = apart = (width, (width // BLOCK + 15) & ~15)
         made.codes = torch.empty_strided((rows, width), (width, 1), dtype=torch.float8_e4m3fn, device=device)      # the quickest of torch's allocations
         made.scales = torch.empty_strided((rows, width // BLOCK), (apart[1], 1), dtype=torch.float8_e8m0fnu, device=device)
         return made

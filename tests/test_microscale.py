@@ -111,9 +111,9 @@ def test_rows_are_laid_out_as_the_kernels_read_them(T, K):
         for s in (scales, scales.t().contiguous().t()):
             rows = Rows8(c, s)
             assert rows.shape == (T, K) and torch.equal(rows.codes.float(), codes.float()) and torch.equal(rows.scales.float(), scales.float())
-            assert rows.codes.data_ptr() % 16 == 0 and rows.scales.data_ptr() % 4 == 0
+            assert rows.codes.data_ptr() % 16 == 0 and rows.scales.data_ptr() % 16 == 0
             if T > 1:
-                assert rows.codes.stride(0) % 16 == 0 and rows.scales.stride(0) % 4 == 0
+                assert rows.codes.stride(0) % 16 == 0 and rows.scales.stride(0) % 16 == 0
             want = codes.float() * scales.float().repeat_interleave(32, dim=1)
             assert torch.equal(rows.decoded(), want)
     made = Rows8.empty(T, K, "cpu")
