@@ -358,9 +358,15 @@ struct ManyShape {
   int BN, stages, m_tiles, n_tiles;
   int w_blocks;                  // groups of 128 features in a tile, the last one not full perhaps
   int w_touched;                 // aligned groups of 128 features that a tile touches at most
-  int vec;                       // runs of features may be moved in 16-byte pieces
+  int vec;                       // runs of 16 features start on 32-byte boundaries
   int smem;
 };
+
+// Eight words on a 32-byte boundary in one store: a whole sector of a lane's row, where two stores of half would be sent one by one.
+__device__ __forceinline__ void store_32(void* at, const uint32_t* p) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]), "r"(p[4]), "r"(p[5]),
+               "r"(p[6]), "r"(p[7]) : "memory");
+}
 
 // 16 features n ... of row t, linear.
 template <int ACT>
@@ -393,13 +399,13 @@ __device__ __forceinline__ void finish_features(const Args& a, int vec, int t, i
         const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
         p[j] = *reinterpret_cast<const uint32_t*>(&two);
       }
-      uint4* c = reinterpret_cast<uint4*>((__nv_bfloat16*)a.C + at);
-      c[0] = make_uint4(p[0], p[1], p[2], p[3]);
-      c[1] = make_uint4(p[4], p[5], p[6], p[7]);
+      store_32((__nv_bfloat16*)a.C + at, p);
     } else {
-      float4* c = reinterpret_cast<float4*>((float*)a.C + at);
+      uint32_t p[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      for (int j = 0; j < 16; ++j) p[j] = __float_as_uint(v[j]);
+      store_32((float*)a.C + at, p);
+      store_32((float*)a.C + at + 8, p + 8);
     }
     return;
   }
@@ -430,9 +436,7 @@ __device__ __forceinline__ void finish_block(const Args& a, int t, int n, const 
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     p[j] = e4m3_pair(v[4 * j] * inverse, v[4 * j + 1] * inverse) | (e4m3_pair(v[4 * j + 2] * inverse, v[4 * j + 3] * inverse) << 16);
-  uint4* c = reinterpret_cast<uint4*>((uint8_t*)a.C + (size_t)t * a.N + n);
-  c[0] = make_uint4(p[0], p[1], p[2], p[3]);
-  c[1] = make_uint4(p[4], p[5], p[6], p[7]);
+  store_32((uint8_t*)a.C + (size_t)t * a.N + n, p);
   a.out_scales[(size_t)t * a.out_scale_stride + n / MX_BLOCK] = (uint8_t)code;
 }
 
@@ -817,7 +821,7 @@ ManyShape many_shape(int T, int N, int K, int vec) {
 
 template <bool GATED>
 int launch_many(const void* codes0, const void* codes1, const void* a, long long a_stride, const Args& args, const char* name, cudaStream_t stream) {
-  const bool vec = args.N % 8 == 0 && (uintptr_t)args.C % 16 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 16 == 0;
+  const bool vec = args.N % 16 == 0 && (uintptr_t)args.C % 32 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 16 == 0;
   const ManyShape s = many_shape<GATED>(args.T, args.N, args.K, vec);
   const long long tiles = (long long)s.m_tiles * s.n_tiles;
   AYK_REQUIRE(tiles <= 0x7fffffff - 65536, "%s: too many rows (%d) and columns (%d)", name, args.T, args.N);
@@ -895,7 +899,7 @@ AYK_EXPORT int ayk_gated_linear4(void* out, void* out_scales, long long out_scal
   args.a_scales = (const uint8_t*)a_scales; args.a_scale_stride = a_scale_stride;
   args.w_scales[0] = (const uint8_t*)gate_scales; args.w_scales[1] = (const uint8_t*)up_scales; args.error = g_error_dev;
   args.T = (int)T; args.N = N; args.K = K; args.n_blocks = (N + TILE_N - 1) / TILE_N; args.act = act;
-  AYK_REQUIRE((uintptr_t)out % 16 == 0, "ayk_gated_linear4: codes must lie on 16-byte boundaries");
+  AYK_REQUIRE((uintptr_t)out % 32 == 0, "ayk_gated_linear4: codes must lie on 32-byte boundaries");
   if (T > FEW_ROWS) return launch_many<true>(gate_codes, up_codes, a, a_stride, args, "ayk_gated_linear4", stream);
   const int bt = T <= 16 ? 16 : T <= 32 ? 32 : 64;
   CUtensorMap mg, mu, ma;
