@@ -194,15 +194,16 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
       }
       pdl_wait();
       for (int i = 0; i < pre; ++i) load_rows(i, i);
-      int issued = pre;
+      int issued = pre, s = 0;
+      uint32_t parity = 0;
       for (int i = pre; i < num_kb; ++i) {
-        const int s = i % STAGES;
-        ok = mbar_wait(empty_bar(s), ((uint32_t)(i / STAGES) & 1u) ^ 1u, args.error, 101);
+        ok = mbar_wait_short(empty_bar(s), parity, args.error, 101);
         if (!ok) break;
         mbar_expect_tx(full_bar(s), L::TX);
         load_weights(i, s);
         load_rows(i, s);
         issued = i + 1;
+        if (++s == STAGES) { s = 0; parity ^= 1u; }
       }
       if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued
         for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(full_bar(i % STAGES), (uint32_t)(i / STAGES) & 1u, args.error, 102);
@@ -212,27 +213,36 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
     cluster_wait();
   } else if (warp == 1) {
     if (elect_one()) {
+      const uint64_t weights0 = make_desc(tiles), rows0 = make_desc(tiles + MATRICES * W_BYTES), w_scales0 = make_desc_scales(w_scales), row_scales0 = make_desc_scales(row_ring);
+      uint32_t bar = full_bar(0), at = 0, scales_at = 0, columns = tmem + L::ACCUMULATORS, parity = 0;      // this stage's: barrier, 16-byte units from the first on, scales
+      uint32_t q = 0, quad_parity = 0;
       for (int i = 0; i < num_kb; ++i) {
-        const int s = i % STAGES, q = (i >> 2) % QUADS;
-        if ((i & 3) == 0) ok = mbar_wait(scales_full(q), (uint32_t)(i / (4 * QUADS)) & 1u, args.error, 103);
-        ok = ok && mbar_wait(full_bar(s), (uint32_t)(i / STAGES) & 1u, args.error, 104);
+        if ((i & 3) == 0) ok = mbar_wait_short(scales_full(q), quad_parity, args.error, 103);
+        ok = ok && mbar_wait_short(bar, parity, args.error, 104);
         if (!ok) break;
         tc_fence_after();
         // A stage's scales have columns of their own: by the time the stage comes round again the MMAs that read them are done.
-        const uint32_t columns = tmem + L::ACCUMULATORS + s * L::SCALE_COLUMNS;
-        tmem_cp_scales(columns, make_desc_scales(row_ring + q * QUAD_BYTES + (i & 3) * SCALE_BYTES));
-        for (int m = 0; m < MATRICES; ++m) tmem_cp_scales(columns + 4 * (m + 1), make_desc_scales(w_scales + (s * MATRICES + m) * SCALE_BYTES));
-        const uint32_t at = tiles + s * L::TILE_BYTES;
-        const uint64_t rows = make_desc(at + MATRICES * W_BYTES);
+        tmem_cp_scales(columns, row_scales0 + (uint64_t)(q * (QUAD_BYTES >> 4) + (i & 3) * (SCALE_BYTES >> 4)));
+#pragma unroll
+        for (int m = 0; m < MATRICES; ++m) tmem_cp_scales(columns + 4 * (m + 1), w_scales0 + scales_at + (uint64_t)(m * (SCALE_BYTES >> 4)));
+        const uint64_t weights = weights0 + at, rows = rows0 + at;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
 #pragma unroll
           for (int m = 0; m < MATRICES; ++m)
-            umma_mx(tmem + m * BT, make_desc(at + m * W_BYTES) + (uint64_t)(2 * k), rows + (uint64_t)(2 * k), idesc_mx_block(IDESC, k),
-                    columns + 4 * (m + 1), columns, (i > 0 || k > 0) ? 1u : 0u);
+            umma_mx(tmem + m * BT, weights + (uint64_t)(m * (W_BYTES >> 4) + 2 * k), rows + (uint64_t)(2 * k), idesc_mx_block(IDESC, k), columns + 4 * (m + 1), columns,
+                    (i > 0 || k > 0) ? 1u : 0u);
         }
-        umma_commit(empty_bar(s));
-        if ((i & 3) == 3) umma_commit(scales_empty(q));
+        umma_commit(bar + 8u * STAGES);
+        bar += 8u;
+        at += L::TILE_BYTES >> 4;
+        scales_at += MATRICES * (SCALE_BYTES >> 4);
+        columns += L::SCALE_COLUMNS;
+        if (bar == full_bar(STAGES)) { bar = full_bar(0); at = scales_at = 0; columns = tmem + L::ACCUMULATORS; parity ^= 1u; }
+        if ((i & 3) == 3) {
+          umma_commit(scales_empty(q));
+          if (++q == QUADS) { q = 0; quad_parity ^= 1u; }
+        }
       }
       umma_commit(done_bar);     // arrives when every MMA issued so far is done
     }
