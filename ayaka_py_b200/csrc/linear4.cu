@@ -752,22 +752,84 @@ int encode_weight(CUtensorMap* map, const void* p, int rows, int K, int box) {
   return 0;
 }
 
-// CTAs along K: as many as fill every multiprocessor's places, with four column blocks for each at least.
-int few_splits(int tiles, int blocks_k, int places, int most) {
+// ----------------------------------------------------------------- choices --
+// Rows and CTAs along K of a launch of the few-row kernel: as many as fill every multiprocessor's places, with two column blocks for
+// each at least; of a gated product one, whose epilogue is the longer part of a short product and is shared among them too (measured
+// with at least 1, 2, 3, 4 blocks, us: 8 x 1024 x 4096 4.25, 3.29, 3.71, 3.70; 16 x 768 x 768 2.99, 3.39, 3.39, 3.29; gated 16 x 768 x
+// 768 3.83, 4.72, 4.69, 5.44; gated 32 x 512 x 2048 4.73, 6.16, 6.88, 6.90).
+template <int BT, bool GATED>
+constexpr int MOST_SPLITS = GATED && BT >= 64 ? 4 : 8;           // what the sums leave of shared memory
+
+template <int BT, bool GATED>
+int few_splits(int T, int N, int K, int sms) {
+  const long long tiles = (long long)((N + TILE_N - 1) / TILE_N) * ((T + BT - 1) / BT);
+  const int blocks = (K + BLOCK_K - 1) / BLOCK_K, least = GATED ? 1 : 2;
   int s = 1;
-  while (2 * s <= most && tiles * 2 * s <= places * ayk_sm_count() && blocks_k >= 4 * 2 * s) s *= 2;
+  while (2 * s <= MOST_SPLITS<BT, GATED> && tiles * 2 * s <= Few<BT, GATED>::PLACES * sms && blocks >= least * 2 * s) s *= 2;
   return s;
+}
+
+// Microseconds of the two kernels, fitted to graphs of 20 launches each on a B200 (N and K from 768 to 16384, 65 to 1024 rows; off by
+// up to 20 %): per wave of CTAs a fixed part and one per column block.  Both sides of the choice, us few / many: 128 x 6400 x 1600 7.4
+// / 16.6, 512 x 6400 x 1600 14.9 / 17.6, 1024 x 6400 x 1600 29.7 / 18.4, 128 x 4096 x 16384 21.9 / 13.6, gated 256 x 4096 x 4096 17.6 /
+// 16.5, gated 128 x 16384 x 4096 28.6 / 48.3.
+template <bool GATED>
+double few_us(int T, int N, int K, int sms) {
+  const int splits = few_splits<64, GATED>(T, N, K, sms), blocks = (K + BLOCK_K - 1) / BLOCK_K;
+  const long long ctas = (long long)((N + TILE_N - 1) / TILE_N) * ((T + 63) / 64) * splits;
+  return 1.2 + (double)((ctas + sms - 1) / sms) * ((GATED ? 5.0 : 3.2) + (GATED ? 0.335 : 0.22) * ((blocks + splits - 1) / splits));
+}
+
+// The many-row kernel's tile width, with its time: wider tiles cost less a feature and fill the last wave less.
+template <bool GATED>
+ManyShape many_shape(int T, int N, int K, int sms, double* us) {
+  constexpr int MATRICES = GATED ? 2 : 1;
+  const int widths[6] = {224, 192, 128, 96, 64, 32};
+  const int blocks = (K + BLOCK_K - 1) / BLOCK_K;
+  ManyShape best{};
+  *us = 0;
+  for (int i = GATED ? 3 : 0; i < 6; ++i) {
+    ManyShape s{};
+    s.BN = widths[i];
+    s.m_tiles = (T + TILE_T - 1) / TILE_T;
+    s.n_tiles = (N + s.BN - 1) / s.BN;
+    s.w_blocks = (s.BN + TILE_N - 1) / TILE_N;
+    s.w_touched = ((TILE_N % s.BN == 0 ? 0 : s.BN == 192 ? 64 : 96) + s.BN + TILE_N - 1) / TILE_N;      // a tile starts so far behind a group at most
+    const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K, groups = 1 + MATRICES * s.w_blocks;
+    s.smem = 1024 + MANY_QUADS * (groups + 1 + MATRICES * s.w_touched) * QUAD_BYTES + 256;
+    s.stages = (232448 - s.smem) / stage;
+    if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * groups);      // columns of scales
+    if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;
+    s.smem += s.stages * stage;
+    const long long tiles = (long long)s.m_tiles * s.n_tiles;
+    const double block = GATED ? 0.33 + 0.0012 * s.BN : 0.262 + 0.00057 * s.BN;
+    const double time = 2.5 + 0.005 * s.BN + (double)((tiles + sms - 1) / sms) * blocks * block;
+    if (*us == 0 || time < *us) {
+      best = s;
+      *us = time;
+    }
+  }
+  return best;
+}
+
+// Up to 64 rows every weight byte goes by once in the few-row kernel; above, the quicker one.
+template <bool GATED>
+bool takes_few(int T, int N, int K, int sms) {
+  double many;
+  if (T <= 64) return true;
+  many_shape<GATED>(T, N, K, sms, &many);
+  return few_us<GATED>(T, N, K, sms) < many;
 }
 
 template <int BT, bool GATED>
 int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& a, const Args& args, const char* name, cudaStream_t stream) {
   using L = Few<BT, GATED>;
-  constexpr int MOST = GATED && BT >= 64 ? 4 : 8;                // splits; what their sums leave of shared memory
+  constexpr int MOST = MOST_SPLITS<BT, GATED>;
   static_assert(L::smem(MOST) <= 232448 && L::smem(1) <= 232448, "shared memory");
   static_assert(L::USED <= 512 && 8 * (2 * L::STAGES + 2 * MANY_QUADS + 2) <= 256 && L::AT_BARS % 16 == 0, "layout");
   const int tiles_n = (args.N + TILE_N - 1) / TILE_N, tiles_t = (args.T + BT - 1) / BT;
   AYK_REQUIRE(tiles_t <= 65535, "%s: too many rows (%d)", name, args.T);
-  const int splits = few_splits(tiles_n * tiles_t, (args.K + BLOCK_K - 1) / BLOCK_K, L::PLACES, MOST);
+  const int splits = few_splits<BT, GATED>(args.T, args.N, args.K, ayk_sm_count());
   static AykPerDevice configured;
   {
     std::lock_guard<std::mutex> lock(g_mutex);
@@ -795,44 +857,12 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
   return ayk_check_launch(name);
 }
 
-// Width of a tile by the time of its column blocks (clocks: what the stage's bytes take through shared memory, in and out, at 128
-// a clock) and the waves that the tiles make.
-template <bool GATED>
-ManyShape many_shape(int T, int N, int K, int vec) {
-  constexpr int MATRICES = GATED ? 2 : 1;
-  const int widths[6] = {224, 192, 128, 96, 64, 32};
-  const int sms = ayk_sm_count(), num_kb = (K + BLOCK_K - 1) / BLOCK_K;
-  ManyShape best{};
-  double best_time = 0;
-  for (int i = GATED ? 3 : 0; i < 6; ++i) {
-    ManyShape s{};
-    s.BN = widths[i];
-    s.m_tiles = (T + TILE_T - 1) / TILE_T;
-    s.n_tiles = (N + s.BN - 1) / s.BN;
-    s.w_blocks = (s.BN + TILE_N - 1) / TILE_N;
-    s.w_touched = ((TILE_N % s.BN == 0 ? 0 : s.BN == 192 ? 64 : 96) + s.BN + TILE_N - 1) / TILE_N;      // a tile starts so far behind a group at most
-    s.vec = vec;
-    const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K, groups = 1 + MATRICES * s.w_blocks;
-    s.smem = 1024 + MANY_QUADS * (groups + 1 + MATRICES * s.w_touched) * QUAD_BYTES + 256;
-    s.stages = (232448 - s.smem) / stage;
-    if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * groups);
-    if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;
-    s.smem += s.stages * stage;
-    const long long tiles = (long long)s.m_tiles * s.n_tiles;
-    const double block = (2.0 * ROWS_BYTES + MATRICES * 1.5 * s.BN * BLOCK_K) / 128;
-    const double time = (double)((tiles + sms - 1) / sms) * num_kb * block + 20.0 * MATRICES * s.BN;
-    if (best_time == 0 || time < best_time) {
-      best = s;
-      best_time = time;
-    }
-  }
-  return best;
-}
-
 template <bool GATED>
 int launch_many(const void* codes0, const void* codes1, const void* a, long long a_stride, const Args& args, const char* name, cudaStream_t stream) {
   const bool vec = args.N % 16 == 0 && (uintptr_t)args.C % 32 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 16 == 0;
-  const ManyShape s = many_shape<GATED>(args.T, args.N, args.K, vec);
+  double us;
+  ManyShape s = many_shape<GATED>(args.T, args.N, args.K, ayk_sm_count(), &us);
+  s.vec = vec;
   const long long tiles = (long long)s.m_tiles * s.n_tiles;
   AYK_REQUIRE(tiles <= 0x7fffffff - 65536, "%s: too many rows (%d) and columns (%d)", name, args.T, args.N);
   CUtensorMap w0, w1, rows, row_scales;
@@ -856,8 +886,6 @@ int launch_many(const void* codes0, const void* codes1, const void* a, long long
   return ayk_check_launch(name);
 }
 
-constexpr int FEW_ROWS = 64;
-
 int check(const char* name, const void* a, long long a_stride, const void* a_scales, long long a_scale_stride, long long T, int N, int K, int act) {
   AYK_REQUIRE(N > 0 && K > 0 && K % MX_BLOCK == 0, "%s: a product of %d columns over rows of %d (whole blocks of %d)", name, N, K, MX_BLOCK);
   AYK_REQUIRE(T >= 0 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256, "%s: too many rows (%lld) or columns (%d)", name, T, N);
@@ -871,6 +899,20 @@ int check(const char* name, const void* a, long long a_stride, const void* a_sca
 
 AYK_EXPORT int ayk_linear4_error() { return g_error_host ? *g_error_host : 0; }
 AYK_EXPORT void ayk_linear4_clear_error() { if (g_error_host) *g_error_host = 0; }
+
+// What a product of these sizes runs as: rows of a tile (16, 32 or 64: the few-row kernel, with `parts` CTAs along K to a tile; 128:
+// the many-row kernel, with tiles `parts` features wide).  Host arithmetic.
+AYK_EXPORT int ayk_linear4_plan(int T, int N, int K, int gated, int sms, int* parts) {
+  double us;
+  if (!(gated ? takes_few<true>(T, N, K, sms) : takes_few<false>(T, N, K, sms))) {
+    *parts = gated ? many_shape<true>(T, N, K, sms, &us).BN : many_shape<false>(T, N, K, sms, &us).BN;
+    return TILE_T;
+  }
+  if (T <= 16) *parts = gated ? few_splits<16, true>(T, N, K, sms) : few_splits<16, false>(T, N, K, sms);
+  else if (T <= 32) *parts = gated ? few_splits<32, true>(T, N, K, sms) : few_splits<32, false>(T, N, K, sms);
+  else *parts = gated ? few_splits<64, true>(T, N, K, sms) : few_splits<64, false>(T, N, K, sms);
+  return T <= 16 ? 16 : T <= 32 ? 32 : 64;
+}
 
 // The arguments come as one block of memory: a call with fifteen of them from Python takes 0.6 us more.
 //
@@ -896,7 +938,7 @@ AYK_EXPORT int ayk_linear4(const Linear4Call* call) {
   args.C = c.C; args.a_scales = (const uint8_t*)c.a_scales; args.a_scale_stride = c.a_scale_stride; args.w_scales[0] = (const uint8_t*)c.scales;
   args.bias = c.bias; args.residual = c.residual; args.error = g_error_dev; args.T = (int)c.T; args.N = c.N; args.K = c.K;
   args.n_blocks = (c.N + TILE_N - 1) / TILE_N; args.act = c.act; args.out_bf16 = c.out_dtype == AYK_DTYPE_BF16;
-  if (c.T > FEW_ROWS) return launch_many<false>(c.codes, c.codes, c.a, c.a_stride, args, "ayk_linear4", c.stream);
+  if (!takes_few<false>(args.T, args.N, args.K, ayk_sm_count())) return launch_many<false>(c.codes, c.codes, c.a, c.a_stride, args, "ayk_linear4", c.stream);
   const int bt = c.T <= 16 ? 16 : c.T <= 32 ? 32 : 64;
   CUtensorMap mw, ma;
   if (encode_weight(&mw, c.codes, args.n_blocks * TILE_N, c.K, TILE_N) != 0 || encode_rows(&ma, c.a, c.T, c.K, c.a_stride, bt) != 0) return -1;
@@ -930,7 +972,7 @@ AYK_EXPORT int ayk_gated_linear4(const GatedLinear4Call* call) {
   args.a_scales = (const uint8_t*)c.a_scales; args.a_scale_stride = c.a_scale_stride;
   args.w_scales[0] = (const uint8_t*)c.gate_scales; args.w_scales[1] = (const uint8_t*)c.up_scales; args.error = g_error_dev;
   args.T = (int)c.T; args.N = c.N; args.K = c.K; args.n_blocks = (c.N + TILE_N - 1) / TILE_N; args.act = c.act;
-  if (c.T > FEW_ROWS) return launch_many<true>(c.gate_codes, c.up_codes, c.a, c.a_stride, args, "ayk_gated_linear4", c.stream);
+  if (!takes_few<true>(args.T, args.N, args.K, ayk_sm_count())) return launch_many<true>(c.gate_codes, c.up_codes, c.a, c.a_stride, args, "ayk_gated_linear4", c.stream);
   const int bt = c.T <= 16 ? 16 : c.T <= 32 ? 32 : 64;
   CUtensorMap mg, mu, ma;
   if (encode_weight(&mg, c.gate_codes, args.n_blocks * TILE_N, c.K, TILE_N) != 0 || encode_weight(&mu, c.up_codes, args.n_blocks * TILE_N, c.K, TILE_N) != 0 ||

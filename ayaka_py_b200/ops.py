@@ -1870,6 +1870,15 @@ def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: 
     return out
 
 
+def linear4_plan(T: int, N: int, K: int, gated: bool = False, sms: int = 148) -> tuple[int, int]:
+    """How ``linear4`` (``gated``: ``gated_linear4``) runs T rows of K columns times N features on ``sms`` SMs: (rows of a tile, parts).
+    16, 32 or 64 rows: the kernel for few rows, with that many CTAs along K to a tile; 128: the one for many, with tiles that many
+    features wide.  Host arithmetic from the kernels' fitted times: works without a GPU."""
+    parts = ctypes.c_int(0)
+    rows = library().ayk_linear4_plan(ctypes.c_int(T), ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(1 if gated else 0), ctypes.c_int(sms), ctypes.byref(parts))
+    return rows, parts.value
+
+
 def gated_linear4(a: Rows8, gate: Matrix4, up: Matrix4, activation: str = "silu") -> Rows8:
     """act(a @ gate^T) * (a @ up^T) in 8 bits: the first half of a gated feed-forward, whose rows the second half's ``linear4``
     reads.  Both products' sums, the activation and their product are 32-bit; the code is the one rounding."""
