@@ -83,6 +83,8 @@ class Matrix4:
                 or tuple(scales.shape) != (kt, nt, TILE * TILE // BLOCK) or scales.dtype != torch.uint8 or not scales.is_contiguous()
                 or N < 1 or K < BLOCK or K % BLOCK or codes.device != scales.device or codes.data_ptr() % 32 or scales.data_ptr() % 16):
             raise FormatError(f"not the blocks of a weight {tuple(shape)}: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
+        if codes.is_cuda:
+            torch.cuda.current_stream(codes.device).synchronize()
         self.codes, self.scales, self.shape = codes, scales, (int(N), int(K))
 
     @classmethod
@@ -105,8 +107,6 @@ class Matrix4:
         s[:N, :K // BLOCK] = scales
         c = c.view(nt * TILE, kt, TILE // 2).transpose(0, 1).clone(memory_format=torch.contiguous_format)
         s = s.view(nt, 4, 32, kt, 4).permute(3, 0, 2, 1, 4).clone(memory_format=torch.contiguous_format).view(kt, nt, TILE * TILE // BLOCK)
-        if c.is_cuda:
-            torch.cuda.current_stream(c.device).synchronize()
         return cls(c, s, (N, K))
 
     def row_major(self) -> tuple[torch.Tensor, torch.Tensor]:

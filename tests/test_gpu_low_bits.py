@@ -283,6 +283,40 @@ def test_a_feed_forward_as_a_block_runs_it(T):
     assert float((x.double() - start).norm()) > 0 and bool(torch.isfinite(x).all())
 
 
+@pytest.mark.parametrize("T", [1, 17, 200])
+@pytest.mark.parametrize("kind", ["mlp", "gated_mlp"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_feed_forward_parts_with_4_bit_weights(dtype, kind, T):
+    """The parts against the same steps in 64 bits over the rounded weights.  Rows are 8-bit: 2^-4 a number at random signs, twice
+    in a row, over the activation between (slope at most 1.13); the outputs' norm takes well under 2^-3 of itself from that."""
+    from ayaka_py_b200.parts import PartSpec, make_part
+    d, inner = 256, 672
+    gen = generator(T)
+    part = make_part(PartSpec(kind, {"width": d, "inner": inner, "activation": "gelu_tanh", "weight_bits": 4}), dtype, "cuda")
+    tensors = {}
+    for name, decl in part.tensors().items():
+        scale = 1 / math.sqrt(decl.shape[1]) if decl.kind == "matrix" else 0.1
+        tensors[name] = (torch.randn(decl.shape, generator=gen, device="cuda") * scale).to(dtype if decl.kind == "matrix" else torch.float32)
+    kept = {name: (matrix4(t).decoded() if t.dim() == 2 else t).double() for name, t in tensors.items()}
+    part.bind(tensors)
+    assert part.join_input(torch.zeros(8, d, device="cuda"), None) is None
+    h = torch.randn(T, d, generator=gen, device="cuda").to(dtype)
+    stream = torch.randn(T, d, generator=gen, device="cuda")
+    before = stream.double()
+    out = part.forward(h, stream, None)
+    assert out is stream
+    act = ACTS["gelu_tanh"]
+    if kind == "mlp":
+        want = act(h.double() @ kept["up_weight"].T + kept["up_bias"]) @ kept["down_weight"].T + kept["down_bias"]
+    else:
+        want = (act(h.double() @ kept["gate_weight"].T) * (h.double() @ kept["up_weight"].T)) @ kept["down_weight"].T
+    got = out.double() - before
+    assert float((got - want).norm() / want.norm()) < 2.0 ** -3
+    if kind == "gated_mlp":
+        alone = part.forward(h, None, None)
+        assert alone.dtype == torch.float32 and float((alone.double() - want).norm() / want.norm()) < 2.0 ** -3
+
+
 @pytest.mark.parametrize("T", [1, 12, 150])
 def test_captured_and_replayed_beside_another_stream(T):
     d, inner = 512, 640

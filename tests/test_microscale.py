@@ -120,6 +120,47 @@ def test_rows_are_laid_out_as_the_kernels_read_them(T, K):
     assert made.shape == (T, K) and made.scales.shape == (T, K // 32) and made.scales.stride(0) == scale_columns(K)
 
 
+@pytest.mark.parametrize("kind,params", [("mlp", {"width": 48, "inner": 64, "activation": "gelu_tanh"}),
+                                         ("gated_mlp", {"width": 64, "inner": 72, "activation": "silu"}),
+                                         ("gated_mlp", {"width": 64, "inner": 64, "activation": "limited_glu"}),
+                                         ("mlp", {"width": 64, "inner": 64, "activation": "gelu_tanh", "weight_bits": 8})])
+def test_feed_forwards_that_cannot_have_4_bit_weights(kind, params):
+    from ayaka_py_b200.parts import PartSpec, make_part
+    with pytest.raises(ValueError):
+        make_part(PartSpec(kind, {"weight_bits": 4, **params}), torch.bfloat16, "cpu")
+
+
+def test_a_part_binds_its_4_bit_weights():
+    from ayaka_py_b200.parts import PartSpec, make_part
+    from ayaka_py_b200.parts.base import NotLowered
+    part = make_part(PartSpec("mlp", {"width": 64, "inner": 96, "activation": "gelu_tanh", "bias": False, "weight_bits": 4}), torch.float32, "cpu")
+    w = {name: torch.randn(decl.shape, generator=torch.Generator().manual_seed(1)) for name, decl in part.tensors().items()}
+    part.bind(w)
+    assert torch.equal(part.up4.decoded(), matrix4(w["up_weight"]).decoded()) and part.down4.shape == (64, 96) and part.up_weight is None
+    with pytest.raises(NotLowered):
+        part.lower(None, 0, 0)
+
+
+# --------------------------------------------------------- the kernels' choices --
+
+def test_choice_of_a_products_kernel():
+    """Measured on both sides: few rows stay with the kernel that streams the weight, which splits K where tiles alone leave
+    multiprocessors idle; many rows go to the persistent one, unless few features and a long K leave that one's tiles too few."""
+    for T in (1, 16, 17, 32, 33, 64):
+        for N, K in ((32, 32), (768, 768), (4096, 16384), (16384, 4096)):
+            for gated in (False, True):
+                rows, parts = ops.linear4_plan(T, N, K, gated)
+                assert rows == (16 if T <= 16 else 32 if T <= 32 else 64) and parts in (1, 2, 4, 8)
+                assert parts <= -(-K // 128) and (parts == 1 or -(-N // 128) * parts <= 296)
+    assert ops.linear4_plan(8, 4096, 16384) == (16, 8) and ops.linear4_plan(61, 6400, 1600) == (64, 2)
+    assert ops.linear4_plan(128, 1600, 6400)[0] == 64 and ops.linear4_plan(1024, 1600, 6400)[0] == 128          # 7.4 / 16.6, 29.7 / 18.4 us
+    assert ops.linear4_plan(128, 16384, 4096)[0] == 128 and ops.linear4_plan(128, 4096, 16384)[0] == 64          # 21.9 / 13.6, 19.6 / 38.5
+    assert ops.linear4_plan(4096, 16384, 4096) == (128, 224) and ops.linear4_plan(4096, 16384, 4096, True) == (128, 96)
+    widths = {ops.linear4_plan(T, N, K)[1] for T in (100, 300, 1000, 3000) for N in (64, 500, 1600, 4096, 9000) for K in (256, 2048)
+              if ops.linear4_plan(T, N, K)[0] == 128}
+    assert widths == {32, 64, 96, 128, 192, 224}                                                                # every width has its products
+
+
 # ------------------------------------------------------- refusals of the calls --
 
 class NoLaunch:
