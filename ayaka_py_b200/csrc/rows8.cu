@@ -168,9 +168,13 @@ int launch(const char* name, uint8_t* codes, uint8_t* scales, long long scale_st
   if (T == 0) return 0;
   auto aligned = [](const void* p, long long stride, size_t size) { return (uintptr_t)p % 16 == 0 && stride * (long long)size % 16 == 0; };
   const int whole = (aligned(x, x_stride, sizeof(X)) ? 1 : 0) | (aligned(y, y_stride, sizeof(Y)) ? 2 : 0) | (aligned(w, 0, 4) ? 4 : 0);
-  // As few numbers to a thread as rows of MOST_THREADS allow: a row is a chain of loads, a sum and stores, and many rows are under way.
-  const int runs = K / RUN;
+  // Few rows: as few runs to a thread as MOST_THREADS allow, for a row is a chain of loads, a sum and stores.  Many rows: 48 bytes of
+  // loads under way to a thread at least (8192 x 4096, us with one, two, four runs to a thread: bfloat16 rows 21.8, 17.9, 16.4, norm
+  // alone 44.7, 35.0, 34.8, norm with y, which has 48 a run, 61.5, 65.9, 63.7).
+  const int runs = K / RUN, bytes = RUN * (int)(sizeof(X) + (y ? sizeof(Y) : 0));
   int items = 1;
+  if (T >= 4 * ayk_sm_count())
+    while (items < MOST_ITEMS && items * bytes < 48 && runs / (2 * items) >= 32) items *= 2;
   while (items <= MOST_ITEMS && (runs + items - 1) / items > MOST_THREADS) items *= 2;
   const int threads = items > MOST_ITEMS ? MOST_THREADS : ((runs + items - 1) / items + 31) / 32 * 32;
   const dim3 block(threads, threads == 32 ? 4 : 1);
