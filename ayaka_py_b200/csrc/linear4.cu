@@ -7,7 +7,7 @@
 // Weights lie in column blocks of 128 (64 bytes of codes a row), their scales beside them as the tensor cores take them.  The
 // copy engine spreads sixteen codes over sixteen bytes on their way into shared memory.
 //
-// Every wait is bounded; one that runs out records a code (101 ... 119) in an error word and the CTA winds down.
+// Every wait is bounded; one that runs out records a code (101 ... 118) in an error word and the CTA winds down.
 #include <cuda.h>
 
 #include <mutex>
@@ -350,18 +350,18 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
 // gated product BN of each matrix), two accumulators in tensor memory so that a tile's epilogue runs under the next one's main
 // loop.  An epilogue thread owns a row and stores runs of features.
 //
-// Scales travel for four column blocks (a quad) at a time, as they lie in memory, and are put in order in shared
-// memory: warp 2 turns the rows', of which 16 bytes come for each row; warp 3 shifts the weights' so that a tile's first feature has
+// Scales travel for four column blocks (a quad) at a time, as they lie in memory.  Four warps, one to a quarter of the lanes of
+// tensor memory, put them there: the rows' turned (16 bytes come for each row), the weights' shifted so that a tile's first feature has
 // the first column (the MMA takes its scales from a whole group of four columns on, and a tile may start at any 32 features).
-// Loaded by those warps themselves, a quad after the other, they set the pace: 0.58 us a column block against 0.3.
+// Copied by tcgen05.cp from shared memory, in order with the MMAs, they held those up: 220 us for 4096 x 4096 x 16384.
 //
-// Warp 0: the operands' copies; warp 1: MMA issue, tensor memory; warps 2, 3: scales; warps 4 ... 11: epilogue, two to a quarter of
-// the rows, each with every other run of features; warp 12: the scales' copies.
+// Warp 0: the operands' copies; warp 1: MMA issue, tensor memory; warps 2, 3, 12, 13: scales; warps 4 ... 11: epilogue, two to a
+// quarter of the rows, each with every other run of features; warp 14: the scales' copies.
 constexpr int TILE_T = 128;
-constexpr int MANY_THREADS = 416;
+constexpr int MANY_THREADS = 480;
 constexpr int ROWS_BYTES = TILE_T * BLOCK_K;
 constexpr int MANY_MOST_STAGES = 8;
-constexpr int MANY_QUADS = 2;                   // places of the two rings, of scales as they come and in order
+constexpr int MANY_QUADS = 2;                   // places of the ring of scales as they come
 constexpr int MANY_MOST_BLOCKS = 3;             // of 128 features' scales that a tile of 224 touches
 
 struct ManyShape {
@@ -465,19 +465,16 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   const int BN = shape.BN, stages = shape.stages;
   const int weight_bytes = BN * BLOCK_K, tile_bytes = ROWS_BYTES + MATRICES * weight_bytes;
-  const int groups = 1 + MATRICES * shape.w_blocks, quad_bytes = groups * QUAD_BYTES;      // a quad: [group][column block][512]
-  const int come_bytes = (1 + MATRICES * shape.w_touched) * QUAD_BYTES;                    // as they come: rows [128][16], features [matrix][group][column block][512]
-  const uint32_t raw = smem_u32(smem_raw), tiles = (raw + 1023u) & ~1023u, ring = tiles + stages * tile_bytes;
-  const uint32_t come = ring + MANY_QUADS * quad_bytes, bars = come + MANY_QUADS * come_bytes;
+  const int groups = 1 + MATRICES * shape.w_blocks;                          // of 128 rows' or features' scales, four columns of tensor memory each
+  const int quad_bytes = (1 + MATRICES * shape.w_touched) * QUAD_BYTES;      // as they come: rows [128][16], features [matrix][column block][group][512]
+  const uint32_t raw = smem_u32(smem_raw), tiles = (raw + 1023u) & ~1023u, come = tiles + stages * tile_bytes, bars = come + MANY_QUADS * quad_bytes;
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (MANY_MOST_STAGES + s); };
-  auto scales_full = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + q); };
-  auto scales_empty = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + MANY_QUADS + q); };
-  auto sums_full = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + b); };
-  auto sums_empty = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + 2 + b); };
-  auto come_full = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 * MANY_QUADS + 4 + q); };
-  auto come_empty = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 3 * MANY_QUADS + 4 + q); };
-  const uint32_t tmem_slot = bars + 8u * (2 * MANY_MOST_STAGES + 4 * MANY_QUADS + 4);
+  auto sums_full = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + b); };
+  auto sums_empty = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 + b); };
+  auto come_full = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 4 + q); };
+  auto come_empty = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 4 + MANY_QUADS + q); };
+  const uint32_t tmem_slot = bars + 8u * (2 * MANY_MOST_STAGES + 4 + 2 * MANY_QUADS);
 
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int num_kb = (args.K + BLOCK_K - 1) / BLOCK_K;
@@ -488,14 +485,12 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     if (GATED) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w1) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
     for (int s = 0; s < stages; ++s) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), 1 + 4);         // the operands' copies and the four warps that bring the scales
       mbar_init(empty_bar(s), 1);
     }
     for (int q = 0; q < MANY_QUADS; ++q) {
-      mbar_init(scales_full(q), 2);
-      mbar_init(scales_empty(q), 1);
       mbar_init(come_full(q), 1);
-      mbar_init(come_empty(q), 2);
+      mbar_init(come_empty(q), 4);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(sums_full(b), 1);
@@ -537,7 +532,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           if (bar == bars_end) { bar = full_bar(0); at = tiles; parity ^= 1u; }
         }
       }
-      if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued
+      if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued (the scales of each come before long)
         for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(full_bar(i % stages), (uint32_t)(i / stages) & 1u, args.error, 112);
       }
     }
@@ -546,21 +541,16 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     if (elect_one()) {
       const uint32_t idesc = make_idesc_mx(TILE_T, BN, MX_E4M3, MX_E2M1);
       const uint32_t bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0), all_sums = 2 * MATRICES * BN;
-      const uint64_t rows0 = make_desc(tiles), weights0 = make_desc(tiles + ROWS_BYTES), scales0 = make_desc_scales(ring);
+      const uint64_t rows0 = make_desc(tiles), weights0 = make_desc(tiles + ROWS_BYTES);
       uint32_t bar = full_bar(0), at = 0, parity = 0, columns = tmem + all_sums;      // this stage's: barrier, 16-byte units from the first on, scales
-      uint32_t q = 0, quad_at = 0, quad_parity = 0;
       int it = 0;
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
         const uint32_t buffer = it & 1, sums = tmem + buffer * MATRICES * BN;
         if (it >= 2) ok = mbar_wait_short(sums_empty(buffer), ((uint32_t)(it >> 1) & 1u) ^ 1u, args.error, 113);
         for (int kb = 0; kb < num_kb && ok; ++kb) {
-          if ((kb & 3) == 0) ok = mbar_wait_short(scales_full(q), quad_parity, args.error, 114);
-          ok = ok && mbar_wait_short(bar, parity, args.error, 115);
+          ok = mbar_wait_short(bar, parity, args.error, 114);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t scales = scales0 + quad_at + (uint64_t)((kb & 3) * (SCALE_BYTES >> 4));
-#pragma unroll 1
-          for (int g = 0; g < groups; ++g) tmem_cp_scales(columns + 4 * g, scales + (uint64_t)(g * (QUAD_BYTES >> 4)));      // a stage's own columns, as above
           const uint64_t rows = rows0 + at, weights = weights0 + at;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -574,17 +564,12 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           at += tile_bytes >> 4;
           columns += 4 * groups;
           if (bar == bars_end) { bar = full_bar(0); at = 0; columns = tmem + all_sums; parity ^= 1u; }
-          if ((kb & 3) == 3 || kb == num_kb - 1) {
-            umma_commit(scales_empty(q));
-            quad_at += quad_bytes >> 4;
-            if (++q == MANY_QUADS) { q = 0; quad_at = 0; quad_parity ^= 1u; }
-          }
         }
         umma_commit(sums_full(buffer));
       }
     }
     __syncwarp();
-  } else if (warp == 12) {
+  } else if (warp == 14) {
     if (elect_one()) {
       int quads = 0;
       pdl_wait();
@@ -596,10 +581,10 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           if (quads >= MANY_QUADS) ok = mbar_wait_short(come_empty(q), ((uint32_t)(quads / MANY_QUADS) & 1u) ^ 1u, args.error, 116);
           if (!ok) break;
           mbar_expect_tx(come_full(q), QUAD_BYTES + MATRICES * kbs * blocks * SCALE_BYTES);
-          tma_load_2d(come + q * come_bytes, &map_s, 4 * first, t0, come_full(q));
+          tma_load_2d(come + q * quad_bytes, &map_s, 4 * first, t0, come_full(q));
           for (int m = 0; m < MATRICES; ++m)
             for (int k = 0; k < kbs; ++k)      // [matrix][column block][group]: a column block's groups lie side by side in memory too
-              bulk_load(come + q * come_bytes + QUAD_BYTES + (m * 4 + k) * shape.w_touched * SCALE_BYTES,
+              bulk_load(come + q * quad_bytes + QUAD_BYTES + (m * 4 + k) * shape.w_touched * SCALE_BYTES,
                         args.w_scales[m] + ((size_t)(first + k) * args.n_blocks + block0) * SCALE_BYTES, blocks * SCALE_BYTES, come_full(q));
         }
       }
@@ -608,50 +593,55 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       }
     }
     __syncwarp();
-  } else if (warp < 4) {
+  } else if (warp < 4 || warp >= 12) {
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 2 * MATRICES * BN, bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0);
+    uint32_t bar = full_bar(0), columns = lanes, parity = 1;       // of the stage: the scales' columns are free when the operands' place is
     int quad = 0;
     for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
       const int shift = tile / shape.m_tiles * BN % TILE_N / 32;
       for (int first = 0; first < num_kb && ok; first += 4, ++quad) {
         const int q = quad % MANY_QUADS;
-        const uint32_t from = come + q * come_bytes + lane * 16, to = ring + q * quad_bytes + lane * 16;
-        ok = mbar_wait(come_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 118);
-        if (ok && quad >= MANY_QUADS) ok = mbar_wait(scales_empty(q), ((uint32_t)(quad / MANY_QUADS) & 1u) ^ 1u, args.error, 119);
+        const uint32_t from = come + q * quad_bytes + lane * 16;
+        ok = mbar_wait(come_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 115);
         if (!ok) break;
-        if (warp == 2) {                     // rows lane, lane + 32, ...: 16 bytes are a row's four column blocks
-          uint32_t w[4][4];
+        uint32_t r[4][4];                    // rows lane, lane + 32, ...: 16 bytes are a row's four column blocks
 #pragma unroll
-          for (int j = 0; j < 4; ++j) lds_v4(from + j * 512, w[j]);
+        for (int j = 0; j < 4; ++j) lds_v4(from + j * 512, r[j]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sts_v4(to + k * SCALE_BYTES, w[0][k], w[1][k], w[2][k], w[3][k]);
-        } else {
-#pragma unroll 1
-          for (int m = 0; m < MATRICES; ++m)
-#pragma unroll 1
-            for (int k = 0; k < 4; ++k) {
-              uint32_t w[4 * MANY_MOST_BLOCKS + 4];                  // this lane's columns of the groups, in a row
+        for (int k = 0; k < 4; ++k) {
+          if (first + k >= num_kb || !ok) continue;
+          ok = mbar_wait(bar + to_empty, parity, args.error, 118);
+          if (!ok) continue;
+          tc_fence_after();
+          tmem_st4(columns, r[0][k], r[1][k], r[2][k], r[3][k]);
 #pragma unroll
-              for (int b = 0; b < MANY_MOST_BLOCKS; ++b)
-                if (b < shape.w_touched) lds_v4(from + QUAD_BYTES + ((m * 4 + k) * shape.w_touched + b) * SCALE_BYTES, w + 4 * b);
+          for (int m = 0; m < MATRICES; ++m) {
+            uint32_t w[4 * MANY_MOST_BLOCKS + 4];                  // this lane's columns of the groups, in a row
 #pragma unroll
-              for (int j = 0; j < 4; ++j) w[4 * MANY_MOST_BLOCKS + j] = 0u;
-              if (shift & 1)
+            for (int g = 0; g < MANY_MOST_BLOCKS; ++g)
+              if (g < shape.w_touched) lds_v4(from + QUAD_BYTES + ((m * 4 + k) * shape.w_touched + g) * SCALE_BYTES, w + 4 * g);
 #pragma unroll
-                for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 1];
-              if (shift & 2)
+            for (int j = 0; j < 4; ++j) w[4 * MANY_MOST_BLOCKS + j] = 0u;
+            if (shift & 1)
 #pragma unroll
-                for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 2];
+              for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 1];
+            if (shift & 2)
 #pragma unroll
-              for (int b = 0; b < MANY_MOST_BLOCKS - 1; ++b)
-                if (b < shape.w_blocks) sts_v4(to + (1 + m * shape.w_blocks + b) * QUAD_BYTES + k * SCALE_BYTES, w[4 * b], w[4 * b + 1], w[4 * b + 2], w[4 * b + 3]);
-            }
+              for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 2];
+#pragma unroll
+            for (int g = 0; g < MANY_MOST_BLOCKS - 1; ++g)
+              if (g < shape.w_blocks) tmem_st4(columns + 4 * (1 + m * shape.w_blocks + g), w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+          bar += 8u;
+          columns += 4 * groups;
+          if (bar == bars_end) { bar = full_bar(0); columns = lanes; parity ^= 1u; }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(scales_full(q));
-          mbar_arrive(come_empty(q));
-        }
+        if (lane == 0) mbar_arrive(come_empty(q));
       }
     }
   } else {
@@ -796,7 +786,7 @@ ManyShape many_shape(int T, int N, int K, int sms, double* us) {
     s.w_blocks = (s.BN + TILE_N - 1) / TILE_N;
     s.w_touched = ((TILE_N % s.BN == 0 ? 0 : s.BN == 192 ? 64 : 96) + s.BN + TILE_N - 1) / TILE_N;      // a tile starts so far behind a group at most
     const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K, groups = 1 + MATRICES * s.w_blocks;
-    s.smem = 1024 + MANY_QUADS * (groups + 1 + MATRICES * s.w_touched) * QUAD_BYTES + 256;
+    s.smem = 1024 + MANY_QUADS * (1 + MATRICES * s.w_touched) * QUAD_BYTES + 256;
     s.stages = (232448 - s.smem) / stage;
     if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * groups);      // columns of scales
     if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;
