@@ -347,8 +347,8 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
 
 // --------------------------------------------------------------- many rows --
 // Persistent CTAs over tiles of 128 rows (the MMA's M side, a row to a lane of tensor memory) by BN features (its N side; of a
-// gated product BN of each matrix), two accumulators in tensor memory so that a tile's epilogue runs under the next one's main
-// loop.  An epilogue thread owns a row and stores runs of features.
+// gated product BN of each matrix, one behind the other), two accumulators in tensor memory so that a tile's epilogue runs under the
+// next one's main loop.  An epilogue thread owns a row and stores runs of features.
 //
 // Scales travel for four column blocks (a quad) at a time, as they lie in memory.  Four warps, one to a quarter of the lanes of
 // tensor memory, put them there: the rows' turned (16 bytes come for each row), the weights' shifted so that a tile's first feature has
@@ -366,7 +366,7 @@ constexpr int MANY_MOST_BLOCKS = 3;             // of 128 features' scales that 
 
 struct ManyShape {
   int BN, stages, m_tiles, n_tiles;
-  int w_blocks;                  // groups of 128 features in a tile, the last one not full perhaps
+  int groups;                    // of four columns of scales: of 128 rows, and of 128 features of the MMA's N side (the last one not full perhaps)
   int w_touched;                 // aligned groups of 128 features that a tile touches at most
   int vec;                       // runs of 16 features start on 32-byte boundaries
   int smem;
@@ -453,10 +453,6 @@ __device__ __forceinline__ void finish_block(const Args& a, int t, int n, const 
 __device__ __forceinline__ void lds_v4(uint32_t at, uint32_t* w) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void sts_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
 template <bool GATED>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
 linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1, const __grid_constant__ CUtensorMap map_a,
@@ -464,8 +460,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   constexpr int MATRICES = GATED ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   const int BN = shape.BN, stages = shape.stages;
-  const int weight_bytes = BN * BLOCK_K, tile_bytes = ROWS_BYTES + MATRICES * weight_bytes;
-  const int groups = 1 + MATRICES * shape.w_blocks;                          // of 128 rows' or features' scales, four columns of tensor memory each
+  const int weight_bytes = BN * BLOCK_K, tile_bytes = ROWS_BYTES + MATRICES * weight_bytes, groups = shape.groups;
   const int quad_bytes = (1 + MATRICES * shape.w_touched) * QUAD_BYTES;      // as they come: rows [128][16], features [matrix][column block][group][512]
   const uint32_t raw = smem_u32(smem_raw), tiles = (raw + 1023u) & ~1023u, come = tiles + stages * tile_bytes, bars = come + MANY_QUADS * quad_bytes;
   auto full_bar = [&](int s) { return bars + 8u * s; };
@@ -539,7 +534,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     __syncwarp();
   } else if (warp == 1) {
     if (elect_one()) {
-      const uint32_t idesc = make_idesc_mx(TILE_T, BN, MX_E4M3, MX_E2M1);
+      const uint32_t idesc = make_idesc_mx(TILE_T, MATRICES * BN, MX_E4M3, MX_E2M1);
       const uint32_t bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0), all_sums = 2 * MATRICES * BN;
       const uint64_t rows0 = make_desc(tiles), weights0 = make_desc(tiles + ROWS_BYTES);
       uint32_t bar = full_bar(0), at = 0, parity = 0, columns = tmem + all_sums;      // this stage's: barrier, 16-byte units from the first on, scales
@@ -553,12 +548,8 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           tc_fence_after();
           const uint64_t rows = rows0 + at, weights = weights0 + at;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-#pragma unroll
-            for (int m = 0; m < MATRICES; ++m)
-              umma_mx(sums + m * BN, rows + (uint64_t)(2 * k), weights + (uint64_t)(m * (weight_bytes >> 4) + 2 * k), idesc_mx_block(idesc, k), columns,
-                      columns + 4 + 4 * m * shape.w_blocks, (kb > 0 || k > 0) ? 1u : 0u);
-          }
+          for (int k = 0; k < 4; ++k)
+            umma_mx(sums, rows + (uint64_t)(2 * k), weights + (uint64_t)(2 * k), idesc_mx_block(idesc, k), columns, columns + 4, (kb > 0 || k > 0) ? 1u : 0u);
           umma_commit(bar + to_empty);
           bar += 8u;
           at += tile_bytes >> 4;
@@ -614,24 +605,28 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           if (!ok) continue;
           tc_fence_after();
           tmem_st4(columns, r[0][k], r[1][k], r[2][k], r[3][k]);
+          uint32_t w[MATRICES][4 * MANY_MOST_BLOCKS + 4];          // this lane's columns of the groups, in a row
 #pragma unroll
           for (int m = 0; m < MATRICES; ++m) {
-            uint32_t w[4 * MANY_MOST_BLOCKS + 4];                  // this lane's columns of the groups, in a row
 #pragma unroll
             for (int g = 0; g < MANY_MOST_BLOCKS; ++g)
-              if (g < shape.w_touched) lds_v4(from + QUAD_BYTES + ((m * 4 + k) * shape.w_touched + g) * SCALE_BYTES, w + 4 * g);
+              if (g < shape.w_touched) lds_v4(from + QUAD_BYTES + ((m * 4 + k) * shape.w_touched + g) * SCALE_BYTES, w[m] + 4 * g);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[4 * MANY_MOST_BLOCKS + j] = 0u;
+            for (int j = 0; j < 4; ++j) w[m][4 * MANY_MOST_BLOCKS + j] = 0u;
             if (shift & 1)
 #pragma unroll
-              for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 1];
+              for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[m][j] = w[m][j + 1];
             if (shift & 2)
 #pragma unroll
-              for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[j] = w[j + 2];
-#pragma unroll
-            for (int g = 0; g < MANY_MOST_BLOCKS - 1; ++g)
-              if (g < shape.w_blocks) tmem_st4(columns + 4 * (1 + m * shape.w_blocks + g), w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+              for (int j = 0; j < 4 * MANY_MOST_BLOCKS; ++j) w[m][j] = w[m][j + 2];
           }
+          if (GATED) {                       // the second matrix's behind the first one's: one, two or three columns on
+#pragma unroll
+            for (int j = 5; j >= 1; --j) w[0][j] = 32 * j < BN ? w[0][j] : BN == 32 ? w[MATRICES - 1][j - 1] : BN == 64 ? w[MATRICES - 1][max(j - 2, 0)] : w[MATRICES - 1][max(j - 3, 0)];
+          }
+#pragma unroll
+          for (int g = 0; g < MANY_MOST_BLOCKS - 1; ++g)
+            if (g < groups - 1) tmem_st4(columns + 4 * (1 + g), w[0][4 * g], w[0][4 * g + 1], w[0][4 * g + 2], w[0][4 * g + 3]);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -783,12 +778,12 @@ ManyShape many_shape(int T, int N, int K, int sms, double* us) {
     s.BN = widths[i];
     s.m_tiles = (T + TILE_T - 1) / TILE_T;
     s.n_tiles = (N + s.BN - 1) / s.BN;
-    s.w_blocks = (s.BN + TILE_N - 1) / TILE_N;
+    s.groups = 1 + (MATRICES * s.BN + TILE_N - 1) / TILE_N;
     s.w_touched = ((TILE_N % s.BN == 0 ? 0 : s.BN == 192 ? 64 : 96) + s.BN + TILE_N - 1) / TILE_N;      // a tile starts so far behind a group at most
-    const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K, groups = 1 + MATRICES * s.w_blocks;
+    const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K;
     s.smem = 1024 + MANY_QUADS * (1 + MATRICES * s.w_touched) * QUAD_BYTES + 256;
     s.stages = (232448 - s.smem) / stage;
-    if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * groups);      // columns of scales
+    if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * s.groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * s.groups);      // columns of scales
     if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;
     s.smem += s.stages * stage;
     const long long tiles = (long long)s.m_tiles * s.n_tiles;
