@@ -127,7 +127,8 @@ launches = 0      # kernels of this library launched so far (graph replays are c
 def _launch(code: int) -> None:
     global launches
     launches += 1
-    _check(code)
+    if code:
+        _check(code)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -1784,6 +1785,9 @@ def linear(a: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
 
 # --------------------------------------- rows in 8 bits, weights in 4 bits --
 
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _elsewhere(name: str, device: int, *tensors: torch.Tensor | None) -> KernelError:
     """Kernels run on the current device's current stream: the first of the tensors that is on another device, as an error."""
     t = next(t for t in tensors if t is not None and t.get_device() != device)
@@ -1797,13 +1801,13 @@ def rows8(x: torch.Tensor) -> Rows8:
     shape, apart = x.shape, x.stride()
     if len(shape) != 2 or shape[1] < BLOCK or shape[1] % BLOCK or apart[1] != 1:
         raise KernelError(f"rows8: rows must be [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(shape)}")
-    (T, K), tag, device = shape, _tag(x.dtype), torch._C._cuda_getDevice()
+    (T, K), tag, device = shape, _tag(x.dtype), _current_device()
     if x.get_device() != device:
         raise _elsewhere("rows8", device, x)
     out = Rows8.empty(T, K, x.device)
     if T:
         _launch(lib.ayk_rows8(_ROWS8(out.codes.data_ptr(), out.scales.data_ptr(), out.apart[1], x.data_ptr(), apart[0] if T > 1 else K, 0, 0, 0, T, K,
-                                     tag, F32, 0.0, torch._C._cuda_getCurrentRawStream(device))))
+                                     tag, F32, 0.0, _current_stream(device))))
     return out
 
 
@@ -1816,7 +1820,7 @@ def rmsnorm_rows8(x: torch.Tensor, weight: torch.Tensor, eps: float, y: torch.Te
     if len(shape) != 2 or x.dtype != torch.float32 or shape[1] < BLOCK or shape[1] % BLOCK or apart[1] != 1:
         raise KernelError(f"rmsnorm_rows8: the stream must be float32 [T, whole blocks of {BLOCK}] with unit column stride, got {tuple(shape)} of {x.dtype}")
     T, K = shape
-    device = torch._C._cuda_getDevice()
+    device = _current_device()
     if _f32(weight, "weight").numel() != K:
         raise KernelError("rmsnorm_rows8: weight must be float32 of the row width")
     tag, y_at, y_apart = F32, 0, 0
@@ -1831,7 +1835,7 @@ def rmsnorm_rows8(x: torch.Tensor, weight: torch.Tensor, eps: float, y: torch.Te
     out = Rows8.empty(T, K, x.device)
     if T:
         _launch(lib.ayk_rows8(_ROWS8(out.codes.data_ptr(), out.scales.data_ptr(), out.apart[1], x.data_ptr(), apart[0] if T > 1 else K, y_at, y_apart,
-                                     weight.data_ptr(), T, K, F32, tag, eps, torch._C._cuda_getCurrentRawStream(device))))
+                                     weight.data_ptr(), T, K, F32, tag, eps, _current_stream(device))))
     return out
 
 
@@ -1841,7 +1845,7 @@ def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: 
     residual (float32; it may be ``out``) in 32-bit."""
     lib = _ready()
     codes = a.codes
-    (T, K), (N, width), device = codes.shape, w.shape, torch._C._cuda_getDevice()
+    (T, K), (N, width), device = codes.shape, w.shape, _current_device()
     if width != K:
         raise KernelError(f"linear4: operands do not fit: rows {(T, K)}, weight {w.shape}")
     act = ACTIVATIONS.get(activation)
@@ -1866,7 +1870,7 @@ def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: 
     if T:
         apart = a.apart
         _launch(lib.ayk_linear4(_LINEAR4(out.data_ptr(), codes.data_ptr(), a.scales.data_ptr(), apart[0], apart[1], w.codes.data_ptr(), w.scales.data_ptr(),
-                                         bias_at, residual_at, T, N, K, act, tag, torch._C._cuda_getCurrentRawStream(device))))
+                                         bias_at, residual_at, T, N, K, act, tag, _current_stream(device))))
     return out
 
 
@@ -1884,7 +1888,7 @@ def gated_linear4(a: Rows8, gate: Matrix4, up: Matrix4, activation: str = "silu"
     reads.  Both products' sums, the activation and their product are 32-bit; the code is the one rounding."""
     lib = _ready()
     codes = a.codes
-    (T, K), (N, width), device = codes.shape, gate.shape, torch._C._cuda_getDevice()
+    (T, K), (N, width), device = codes.shape, gate.shape, _current_device()
     if width != K or up.shape != gate.shape:
         raise KernelError(f"gated_linear4: operands do not fit: rows {(T, K)}, weights {gate.shape} and {up.shape}")
     if N % BLOCK:
@@ -1899,7 +1903,7 @@ def gated_linear4(a: Rows8, gate: Matrix4, up: Matrix4, activation: str = "silu"
         apart = a.apart
         _launch(lib.ayk_gated_linear4(_GATED_LINEAR4(out.codes.data_ptr(), out.scales.data_ptr(), out.apart[1], codes.data_ptr(), a.scales.data_ptr(),
                                                      apart[0], apart[1], gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
-                                                     up.scales.data_ptr(), T, N, K, act, torch._C._cuda_getCurrentRawStream(device))))
+                                                     up.scales.data_ptr(), T, N, K, act, _current_stream(device))))
     return out
 
 
