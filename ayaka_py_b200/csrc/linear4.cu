@@ -368,7 +368,7 @@ struct ManyShape {
   int BN, stages, m_tiles, n_tiles;
   int groups;                    // of four columns of scales: of 128 rows, and of 128 features of the MMA's N side (the last one not full perhaps)
   int w_touched;                 // aligned groups of 128 features that a tile touches at most
-  int vec;                       // runs of 16 features start on 32-byte boundaries
+  int turned;                    // rows of the result start anywhere: not on 32-byte boundaries
   int smem;
 };
 
@@ -378,54 +378,85 @@ __device__ __forceinline__ void store_32(void* at, const uint32_t* p) {
                "r"(p[6]), "r"(p[7]) : "memory");
 }
 
-// 16 features n ... of row t, linear.
+// 16 features n ... of row t, linear, where every row's start on a 32-byte boundary.
 template <int ACT>
-__device__ __forceinline__ void finish_features(const Args& a, int vec, int t, int n, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void finish_features(const Args& a, int t, int n, const uint32_t (&r)[16]) {
   if (t >= a.T) return;
   const size_t at = (size_t)t * a.N + n;
-  if (vec && n + 16 <= a.N) {
-    float v[16];
-    float4 res[4];
-    if (a.residual) {
+  float v[16];
+  float4 res[4];
+  if (a.residual) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const float4*>(a.residual + at)[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float4 b = a.bias ? reinterpret_cast<const float4*>(a.bias + n)[j] : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[4 * j] = __uint_as_float(r[4 * j]) + b.x; v[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + b.y;
-      v[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + b.z; v[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + b.w;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = apply_activation_tc<ACT>(v[j], a.act);
-    if (a.residual) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { v[4 * j] += res[j].x; v[4 * j + 1] += res[j].y; v[4 * j + 2] += res[j].z; v[4 * j + 3] += res[j].w; }
-    }
-    if (a.out_bf16) {
-      uint32_t p[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        p[j] = *reinterpret_cast<const uint32_t*>(&two);
-      }
-      store_32((__nv_bfloat16*)a.C + at, p);
-    } else {
-      uint32_t p[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) p[j] = __float_as_uint(v[j]);
-      store_32((float*)a.C + at, p);
-      store_32((float*)a.C + at + 8, p + 8);
-    }
-    return;
+    for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const float4*>(a.residual + at)[j];
   }
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    if (n + j < a.N) {
-      const float y = apply_activation_tc<ACT>(__uint_as_float(r[j]) + (a.bias ? a.bias[n + j] : 0.f), a.act) + (a.residual ? a.residual[at + j] : 0.f);
-      if (a.out_bf16) ((__nv_bfloat16*)a.C)[at + j] = __float2bfloat16_rn(y);
-      else ((float*)a.C)[at + j] = y;
+  for (int j = 0; j < 4; ++j) {
+    const float4 b = a.bias ? reinterpret_cast<const float4*>(a.bias + n)[j] : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[4 * j] = __uint_as_float(r[4 * j]) + b.x; v[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + b.y;
+    v[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + b.z; v[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + b.w;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = apply_activation_tc<ACT>(v[j], a.act);
+  if (a.residual) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[4 * j] += res[j].x; v[4 * j + 1] += res[j].y; v[4 * j + 2] += res[j].z; v[4 * j + 3] += res[j].w; }
+  }
+  if (a.out_bf16) {
+    uint32_t p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      p[j] = *reinterpret_cast<const uint32_t*>(&two);
     }
+    store_32((__nv_bfloat16*)a.C + at, p);
+  } else {
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) p[j] = __float_as_uint(v[j]);
+    store_32((float*)a.C + at, p);
+    store_32((float*)a.C + at + 8, p + 8);
+  }
+}
+
+// The same for rows that start anywhere: a warp turns its 32 rows (from t0 on), 32 features at a time, in shared memory and writes them row
+// by row, a lane to a feature.  (5000 x 128 x 2001, us: 13.0; lanes that write their own rows, 2 bytes to a sector, 85; pieces of 8
+// bytes shifted into line through shared memory 16.9, whole sectors 27, for a row's ends then take longer than its middle.  2000
+// features, in whole sectors as they are, 6.7.)
+constexpr int TURNED_ROW = 33;                  // words: a column's neighbours are on other banks
+constexpr int TURNED_BYTES = 8 * 32 * TURNED_ROW * 4;
+template <int ACT, typename O>
+__device__ __forceinline__ void finish_turned(const Args& a, uint32_t sums, float* mine, int t0, int n0, int columns) {
+  const int lane = threadIdx.x & 31, rows = min(32, a.T - t0);
+#pragma unroll 1
+  for (int c = 0; c < columns && n0 + c < a.N; c += 32) {
+    uint32_t r[32];
+    tmem_ld32(sums + c, r);                     // of a last half run, what lies behind it too
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) mine[lane * TURNED_ROW + j] = __uint_as_float(r[j]);
+    __syncwarp();
+    const int n = n0 + c + lane;
+    if (c + lane < columns && n < a.N) {
+      const float b = a.bias ? a.bias[n] : 0.f;
+      O* out = (O*)a.C + (size_t)t0 * a.N + n;
+      const float* add = a.residual + (size_t)t0 * a.N + n;
+      for (int first = 0; first < rows; first += 8) {
+        float res[8];
+        if (a.residual) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) res[i] = first + i < rows ? add[(size_t)i * a.N] : 0.f;
+          add += (size_t)8 * a.N;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float y = apply_activation_tc<ACT>(mine[(first + i) * TURNED_ROW + lane] + b, a.act);
+          if (a.residual) y += res[i];
+          if (first + i < rows) *out = from_float<O>(y);
+          out += a.N;
+        }
+      }
+    }
+    __syncwarp();
   }
 }
 
@@ -651,20 +682,27 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         if (!ok) break;
         tc_fence_after();
         const uint32_t sums = tmem + ((uint32_t)(quarter * 32) << 16) + buffer * MATRICES * BN;
-        constexpr int RUN = GATED ? 32 : 16;
+        if constexpr (GATED) {
 #pragma unroll 1
-        for (int c = half * RUN; c < BN && n0 + c < args.N; c += 2 * RUN) {
-          if constexpr (GATED) {
+          for (int c = half * 32; c < BN && n0 + c < args.N; c += 64) {
             uint32_t g[32], u[32];
             tmem_ld32(sums + c, g);
             tmem_ld32(sums + BN + c, u);
             tmem_ld_wait();
             finish_block<ACT>(args, t, n0 + c, g, u);
-          } else {
+          }
+        } else if (shape.turned) {
+          float* mine = (float*)(smem_raw + (bars + 256 - raw)) + (warp - 4) * 32 * TURNED_ROW;
+          const int from = half * (BN / 2);
+          if (args.out_bf16) finish_turned<ACT, __nv_bfloat16>(args, sums + from, mine, t - lane, n0 + from, BN / 2);
+          else finish_turned<ACT, float>(args, sums + from, mine, t - lane, n0 + from, BN / 2);
+        } else {
+#pragma unroll 1
+          for (int c = half * 16; c < BN && n0 + c < args.N; c += 32) {
             uint32_t r[16];
             tmem_ld16(sums + c, r);
             tmem_ld_wait();
-            finish_features<ACT>(args, shape.vec, t, n0 + c, r);
+            finish_features<ACT>(args, t, n0 + c, r);
           }
         }
         tc_fence_before();
@@ -767,7 +805,7 @@ double few_us(int T, int N, int K, int sms) {
 
 // The many-row kernel's tile width, with its time: wider tiles cost less a feature and fill the last wave less.
 template <bool GATED>
-ManyShape many_shape(int T, int N, int K, int sms, double* us) {
+ManyShape many_shape(int T, int N, int K, int sms, int turned, double* us) {
   constexpr int MATRICES = GATED ? 2 : 1;
   const int widths[6] = {224, 192, 128, 96, 64, 32};
   const int blocks = (K + BLOCK_K - 1) / BLOCK_K;
@@ -781,7 +819,8 @@ ManyShape many_shape(int T, int N, int K, int sms, double* us) {
     s.groups = 1 + (MATRICES * s.BN + TILE_N - 1) / TILE_N;
     s.w_touched = ((TILE_N % s.BN == 0 ? 0 : s.BN == 192 ? 64 : 96) + s.BN + TILE_N - 1) / TILE_N;      // a tile starts so far behind a group at most
     const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K;
-    s.smem = 1024 + MANY_QUADS * (1 + MATRICES * s.w_touched) * QUAD_BYTES + 256;
+    s.turned = turned;
+    s.smem = 1024 + MANY_QUADS * (1 + MATRICES * s.w_touched) * QUAD_BYTES + 256 + (turned ? TURNED_BYTES : 0);
     s.stages = (232448 - s.smem) / stage;
     if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * s.groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * s.groups);      // columns of scales
     if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;
@@ -802,7 +841,7 @@ template <bool GATED>
 bool takes_few(int T, int N, int K, int sms) {
   double many;
   if (T <= 64) return true;
-  many_shape<GATED>(T, N, K, sms, &many);
+  many_shape<GATED>(T, N, K, sms, 0, &many);
   return few_us<GATED>(T, N, K, sms) < many;
 }
 
@@ -844,10 +883,9 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
 
 template <bool GATED>
 int launch_many(const void* codes0, const void* codes1, const void* a, long long a_stride, const Args& args, const char* name, cudaStream_t stream) {
-  const bool vec = args.N % 16 == 0 && (uintptr_t)args.C % 32 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 16 == 0;
+  const bool turned = !GATED && !(args.N % 16 == 0 && (uintptr_t)args.C % 32 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 16 == 0);
   double us;
-  ManyShape s = many_shape<GATED>(args.T, args.N, args.K, ayk_sm_count(), &us);
-  s.vec = vec;
+  const ManyShape s = many_shape<GATED>(args.T, args.N, args.K, ayk_sm_count(), turned, &us);
   const long long tiles = (long long)s.m_tiles * s.n_tiles;
   AYK_REQUIRE(tiles <= 0x7fffffff - 65536, "%s: too many rows (%d) and columns (%d)", name, args.T, args.N);
   CUtensorMap w0, w1, rows, row_scales;
@@ -890,7 +928,7 @@ AYK_EXPORT void ayk_linear4_clear_error() { if (g_error_host) *g_error_host = 0;
 AYK_EXPORT int ayk_linear4_plan(int T, int N, int K, int gated, int sms, int* parts) {
   double us;
   if (!(gated ? takes_few<true>(T, N, K, sms) : takes_few<false>(T, N, K, sms))) {
-    *parts = gated ? many_shape<true>(T, N, K, sms, &us).BN : many_shape<false>(T, N, K, sms, &us).BN;
+    *parts = gated ? many_shape<true>(T, N, K, sms, 0, &us).BN : many_shape<false>(T, N, K, sms, N % 16 != 0, &us).BN;
     return TILE_T;
   }
   if (T <= 16) *parts = gated ? few_splits<16, true>(T, N, K, sms) : few_splits<16, false>(T, N, K, sms);

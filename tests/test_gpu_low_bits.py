@@ -250,6 +250,33 @@ def test_rows_of_any_layout(T):
         assert torch.equal(ops.linear4(rows, w, out_dtype=torch.float32), want)
 
 
+@pytest.mark.parametrize("T,N,K", [(5, 200, 160), (130, 77, 160), (300, 301, 288), (270, 130, 96), (257, 1008, 544)])
+@pytest.mark.parametrize("at,residual_at", [(0, 0), (1, 0), (2, 2), (3, 1), (4, 8), (8, 3)])
+def test_results_and_residuals_that_start_anywhere(T, N, K, at, residual_at):
+    """Rows of the result and of the residual from any number on, next to others that stay as they are."""
+    gen = generator(N)
+    a, w = random_rows(T, K, 1), random_matrix(N, K, 2)
+    bias = torch.randn(N, generator=gen, device="cuda")
+    z, bound = product64(a, w)
+    residual = torch.randn(residual_at + T * N, generator=gen, device="cuda")[residual_at:].view(T, N)
+    y, slack = z + bias.double(), bound + 2.0 ** -23 * (z.abs() + bias.double().abs())
+    for dtype in (torch.float32, torch.bfloat16):
+        for r in (None, residual):
+            store = torch.full((at + T * N + 9,), 7.0, dtype=dtype, device="cuda")
+            out = store[at:at + T * N].view(T, N)
+            ops.linear4(a, w, bias, residual=r, out_dtype=dtype, out=out)
+            want = y if r is None else y + r.double()
+            allowed = slack + 2.0 ** -23 * want.abs() + (0 if r is None else 2.0 ** -23 * r.double().abs())
+            if dtype == torch.bfloat16:
+                allowed = allowed + 2.0 ** -8 * (want.abs() + allowed)
+            assert bool(((out.double() - want).abs() <= allowed).all())
+            assert bool((store[:at] == 7.0).all()) and bool((store[at + T * N:] == 7.0).all())
+    stream = torch.cat((torch.full((at,), 7.0, device="cuda"), residual.reshape(-1)))
+    inside = stream[at:].view(T, N)
+    ops.linear4(a, w, bias, "none", inside, torch.float32, inside)
+    assert torch.equal(inside, ops.linear4(a, w, bias, "none", residual, torch.float32)) and bool((stream[:at] == 7.0).all())
+
+
 @pytest.mark.parametrize("T,N,K", [(3, 200, 160), (130, 200, 160)])
 def test_what_lies_behind_the_rows_is_left_alone(T, N, K):
     a, w = random_rows(T, K, 1), random_matrix(N, K, 2)
