@@ -89,6 +89,7 @@ __device__ __forceinline__ void with_activation(int act, Run run) {
   if (act == AYK_ACT_NONE) run(std::integral_constant<int, AYK_ACT_NONE>());
   else if (act == AYK_ACT_SILU) run(std::integral_constant<int, AYK_ACT_SILU>());
   else if (act == AYK_ACT_GELU_TANH) run(std::integral_constant<int, AYK_ACT_GELU_TANH>());
+  else if (act == AYK_ACT_RELU2) run(std::integral_constant<int, AYK_ACT_RELU2>());
   else run(std::integral_constant<int, -1>());
 }
 
