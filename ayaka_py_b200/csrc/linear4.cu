@@ -119,8 +119,9 @@ struct Few {
   static constexpr int AT_ROW_SCALES = AT_W_SCALES + STAGES * MATRICES * SCALE_BYTES;
   static constexpr int AT_BARS = AT_ROW_SCALES + QUADS * QUAD_BYTES;
   static constexpr int AT_SUMS = AT_BARS + 256;
-  static constexpr int owners(int splits) { return GATED && splits > 4 ? 4 : splits; }       // of a tile's features; a block of 32 has one
-  static constexpr int sums_bytes(int splits) { return MATRICES * splits * (TILE_N / owners(splits)) * BT * 4; }
+  // features of a tile that one CTA of the cluster finishes; of a gated product whole blocks of 32, so that some CTAs may finish none
+  __host__ __device__ static constexpr int share(int splits) { return GATED ? (splits >= 4 ? 32 : splits >= 2 ? 64 : 128) : (TILE_N + splits - 1) / splits; }
+  static constexpr int sums_bytes(int splits) { return MATRICES * splits * share(splits) * BT * 4; }
   static constexpr int smem(int splits) { return 1024 + AT_SUMS + sums_bytes(splits); }
 };
 
@@ -296,7 +297,7 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
       });
     } else {
       // Sums go to the CTA that finishes their features, [matrix][split][four rows][feature]: neighbouring lanes 16 bytes apart.
-      const int per = TILE_N / L::owners(splits), local = quarter * 32 + lane;
+      const int per = L::share(splits), local = quarter * 32 + lane;
       const uint32_t mine = map_to_cta(sums, (uint32_t)(local / per)) + 16u * (uint32_t)(local % per);
 #pragma unroll
       for (int m = 0; m < MATRICES; ++m) {
@@ -316,24 +317,23 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
   __syncwarp();
   if (splits > 1) {
     cluster_sync_all();          // every sum is where it belongs, and nobody leaves before
-    if (warp >= 2 && z < L::owners(splits)) {
-      const int per = TILE_N / L::owners(splits);
+    if (warp >= 2) {
+      const int per = L::share(splits), mine = min(per, TILE_N - z * per);      // none of a gated product's fifth CTA on
       const float4* part = (const float4*)(smem_raw + (sums - raw));
       with_activation(args.act, [&](auto act) {
 #pragma unroll 1
-        for (int p = threadIdx.x - 64; p < per * (BT / 4); p += L::EPILOGUE) {
-          const int f = p % per, four = p / per, t = t0 + 4 * four, n = n0 + z * per + f;
+        for (int p = threadIdx.x - 64; p < mine * (BT / 4); p += L::EPILOGUE) {
+          const int f = p % mine, four = p / mine, t = t0 + 4 * four, n = n0 + z * per + f;
           if (t >= args.T) break;              // a warp's lanes have the same four rows where a block's scale is made (per >= 32)
           float v[MATRICES][4];
 #pragma unroll
           for (int m = 0; m < MATRICES; ++m) {
             const float4* at = part + ((size_t)m * splits * (BT / 4) + four) * per + f;
             v[m][0] = v[m][1] = v[m][2] = v[m][3] = 0.f;
-#pragma unroll 1
-            for (int y = 0; y < splits; y += 2) {                // in the splits' order, whoever came first
-              const float4 x0 = at[y * (BT / 4) * per], x1 = at[(y + 1) * (BT / 4) * per];
-              v[m][0] += x0.x; v[m][1] += x0.y; v[m][2] += x0.z; v[m][3] += x0.w;
-              v[m][0] += x1.x; v[m][1] += x1.y; v[m][2] += x1.z; v[m][3] += x1.w;
+#pragma unroll 2
+            for (int y = 0; y < splits; ++y) {                   // in the splits' order, whoever came first
+              const float4 x = at[y * (BT / 4) * per];
+              v[m][0] += x.x; v[m][1] += x.y; v[m][2] += x.z; v[m][3] += x.w;
             }
           }
           finish_rows<GATED, decltype(act)::value, 4>(args, t, n, n < args.N, v[0], v[MATRICES - 1]);
@@ -777,20 +777,35 @@ int encode_weight(CUtensorMap* map, const void* p, int rows, int K, int box) {
 }
 
 // ----------------------------------------------------------------- choices --
-// Rows and CTAs along K of a launch of the few-row kernel: as many as fill every multiprocessor's places, with two column blocks for
-// each at least; of a gated product one, whose epilogue is the longer part of a short product and is shared among them too (measured
-// with at least 1, 2, 3, 4 blocks, us: 8 x 1024 x 4096 4.25, 3.29, 3.71, 3.70; 16 x 768 x 768 2.99, 3.39, 3.39, 3.29; gated 16 x 768 x
-// 768 3.83, 4.72, 4.69, 5.44; gated 32 x 512 x 2048 4.73, 6.16, 6.88, 6.90).
+// CTAs along K to a tile of the few-row kernel, 1 ... 8.  The clusters of a launch should run at once: with one CTA to a multiprocessor
+// a B200 of 148 takes so many clusters of 1, 2, ... 8 (the driver's occupancy; a cluster stays within a group of multiprocessors), with
+// two as many as were seen to run side by side (S CTAs of 8 column blocks each: 70 clusters of four 6.3 us, 72 10.0; 33 of eight 6.6, 34
+// 10.0).  Among those, the least time: column blocks one after the other, 0.25 us each (two matrices 0.33), 0.6 for the exchange of the
+// sums, and of a gated product the epilogue, which four CTAs share.  (us with 1, 2, 4, 8: 8 x 4096 x 4096 9.5, 6.6, 5.4, 5.7; 64 x 6400 x
+// 1600 14.4, 10.0, 7.1, 6.3; 50 x 2976 x 4226, 34 tiles, 8.5, 7.2, 11.3, 15.1 and with 3 6.8; gated 16 x 768 x 768 5.4, 3.8, 3.6, 3.4.)
 template <int BT, bool GATED>
 constexpr int MOST_SPLITS = GATED && BT >= 64 ? 4 : 8;           // what the sums leave of shared memory
 
 template <int BT, bool GATED>
+int few_clusters(int splits, int sms) {      // that run at once
+  constexpr int one[8] = {148, 74, 45, 33, 26, 22, 15, 15}, two[8] = {296, 148, 90, 66, 52, 44, 32, 32};
+  return (Few<BT, GATED>::PLACES == 2 ? two : one)[splits - 1] * sms / 148;
+}
+template <int BT, bool GATED>
 int few_splits(int T, int N, int K, int sms) {
   const long long tiles = (long long)((N + TILE_N - 1) / TILE_N) * ((T + BT - 1) / BT);
-  const int blocks = (K + BLOCK_K - 1) / BLOCK_K, least = GATED ? 1 : 2;
-  int s = 1;
-  while (2 * s <= MOST_SPLITS<BT, GATED> && tiles * 2 * s <= Few<BT, GATED>::PLACES * sms && blocks >= least * 2 * s) s *= 2;
-  return s;
+  const int blocks = (K + BLOCK_K - 1) / BLOCK_K;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= MOST_SPLITS<BT, GATED> && s <= blocks; ++s) {
+    if ((s > 1 && tiles > few_clusters<BT, GATED>(s, sms)) || Few<BT, GATED>::smem(s) > 232448) continue;
+    const double us = (GATED ? 0.33 : 0.25) * ((blocks + s - 1) / s) + (s > 1 ? 0.6 : 0) + (GATED ? (1.0 + 0.05 * BT) / (s < 4 ? s : 4) : 0);
+    if (least == 0 || us < least) {
+      best = s;
+      least = us;
+    }
+  }
+  return best;
 }
 
 // Microseconds of the two kernels, fitted to graphs of 20 launches each on a B200 (N and K from 768 to 16384, 65 to 1024 rows; off by
@@ -800,8 +815,8 @@ int few_splits(int T, int N, int K, int sms) {
 template <bool GATED>
 double few_us(int T, int N, int K, int sms) {
   const int splits = few_splits<64, GATED>(T, N, K, sms), blocks = (K + BLOCK_K - 1) / BLOCK_K;
-  const long long ctas = (long long)((N + TILE_N - 1) / TILE_N) * ((T + 63) / 64) * splits;
-  return 1.2 + (double)((ctas + sms - 1) / sms) * ((GATED ? 5.0 : 3.2) + (GATED ? 0.335 : 0.22) * ((blocks + splits - 1) / splits));
+  const long long tiles = (long long)((N + TILE_N - 1) / TILE_N) * ((T + 63) / 64), at_once = few_clusters<64, GATED>(splits, sms);
+  return 1.2 + (double)((tiles + at_once - 1) / at_once) * ((GATED ? 5.0 : 3.2) + (GATED ? 0.335 : 0.22) * ((blocks + splits - 1) / splits));
 }
 
 // The many-row kernel's tile width, with its time: wider tiles cost less a feature and fill the last wave less.
@@ -860,7 +875,8 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
     std::lock_guard<std::mutex> lock(g_mutex);
     bool& done = configured.here();
     if (!done) {
-      const int most = L::smem(MOST) > L::smem(1) ? L::smem(MOST) : L::smem(1);
+      int most = 0;
+      for (int s = 1; s <= MOST; ++s) most = L::smem(s) > most && L::smem(s) <= 232448 ? L::smem(s) : most;
       const cudaError_t err = cudaFuncSetAttribute(linear4_few_kernel<BT, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (err != cudaSuccess) return ayk_fail("%s: shared memory %d: %s", name, most, cudaGetErrorString(err));
       done = true;
