@@ -286,6 +286,43 @@ def test_what_lies_behind_the_rows_is_left_alone(T, N, K):
     assert torch.equal(store[:T], ops.linear4(a, w, out_dtype=torch.float32))
 
 
+@pytest.mark.parametrize("T", [2, 40, 200])
+def test_scales_at_the_ends_of_their_range(T):
+    """Powers of two from 2^-127 to 2^127 on both sides, whose products are ordinary numbers again; and products that are too small."""
+    K, N = 256, 96
+    gen = generator(T)
+    codes = torch.randn(T, K, generator=gen, device="cuda").to(torch.float8_e4m3fn)
+    nibbles = torch.randint(0, 256, (N, K // 2), generator=gen, device="cuda", dtype=torch.uint8)
+    for row, weight in ((0, 250), (1, 254), (254, 0), (253, 2), (127, 127), (0, 0), (0, 127), (10, 100)):
+        a = Rows8(codes, torch.full((T, K // 32), row, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu))
+        w = Matrix4.from_codes(nibbles, torch.full((N, K // 32), weight, dtype=torch.uint8, device="cuda"))
+        x = codes.double() * 2.0 ** (row - 127)
+        m = Matrix4.from_codes(nibbles, torch.full((N, K // 32), 127, dtype=torch.uint8, device="cuda")).decoded().double() * 2.0 ** (weight - 127)
+        z, bound = x @ m.T, (K / 32 + 40) * 2.0 ** -23 * (x.abs() @ m.abs().T)
+        got = ops.linear4(a, w, out_dtype=torch.float32).double()
+        assert bool(((got - z).abs() <= bound + 2.0 ** -126).all()), (row, weight)        # below 2^-126: no worse than zero
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 numbers of a result, and of rows."""
+    T, N, K = 70001, 32000, 32
+    a, w = random_rows(T, K, 1), random_matrix(N, K, 2)
+    got = ops.linear4(a, w)
+    for lo in (0, 67000, T - 40):
+        z, bound = product64(Rows8(a.codes[lo:lo + 40], a.scales[lo:lo + 40]), w)
+        assert bool(((got[lo:lo + 40].double() - z).abs() <= bound + 2.0 ** -8 * (z.abs() + bound)).all())
+    rows = ops.rows8(got)
+    for lo in (0, 67000, T - 40):
+        check_quantised(Rows8(rows.codes[lo:lo + 40], rows.scales[lo:lo + 40]), got[lo:lo + 40])
+    del got
+    z = ops.linear4(Rows8(rows.codes[-9:], rows.scales[-9:]), random_matrix(64, N, 3), out_dtype=torch.float32)
+    want, bound = product64(Rows8(rows.codes[-9:].clone(), rows.scales[-9:].clone()), random_matrix(64, N, 3))
+    assert bool(((z.double() - want).abs() <= bound).all())
+    u = ops.linear4(rows, random_matrix(32, N, 4))
+    want, bound = product64(Rows8(rows.codes[-300:], rows.scales[-300:]), random_matrix(32, N, 4))
+    assert bool(((u[-300:].double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all())
+
+
 @pytest.mark.parametrize("T", [1, 9, 70, 400])
 def test_a_feed_forward_as_a_block_runs_it(T):
     """norm of the stream -> gate, up -> down onto the stream, each step against 64 bits on the rows that the one before made."""
