@@ -379,16 +379,20 @@ __device__ __forceinline__ void store_32(void* at, const uint32_t* p) {
                "r"(p[6]), "r"(p[7]) : "memory");
 }
 
+__device__ __forceinline__ void load_32(const float* at, float* v) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(at) : "memory");
+}
+
 // 16 features n ... of row t, linear, where every row's start on a 32-byte boundary.
 template <int ACT>
 __device__ __forceinline__ void finish_features(const Args& a, int t, int n, const uint32_t (&r)[16]) {
   if (t >= a.T) return;
   const size_t at = (size_t)t * a.N + n;
-  float v[16];
-  float4 res[4];
+  float v[16], res[16];
   if (a.residual) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) res[j] = reinterpret_cast<const float4*>(a.residual + at)[j];
+    load_32(a.residual + at, res);
+    load_32(a.residual + at + 8, res + 8);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -400,7 +404,7 @@ __device__ __forceinline__ void finish_features(const Args& a, int t, int n, con
   for (int j = 0; j < 16; ++j) v[j] = apply_activation_tc<ACT>(v[j], a.act);
   if (a.residual) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { v[4 * j] += res[j].x; v[4 * j + 1] += res[j].y; v[4 * j + 2] += res[j].z; v[4 * j + 3] += res[j].w; }
+    for (int j = 0; j < 16; ++j) v[j] += res[j];
   }
   if (a.out_bf16) {
     uint32_t p[8];
@@ -900,7 +904,7 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
 
 template <bool GATED>
 int launch_many(const void* codes0, const void* codes1, const void* a, long long a_stride, const Args& args, const char* name, cudaStream_t stream) {
-  const bool turned = !GATED && !(args.N % 16 == 0 && (uintptr_t)args.C % 32 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 16 == 0);
+  const bool turned = !GATED && !(args.N % 16 == 0 && (uintptr_t)args.C % 32 == 0 && (uintptr_t)args.bias % 16 == 0 && (uintptr_t)args.residual % 32 == 0);
   double us;
   const ManyShape s = many_shape<GATED>(args.T, args.N, args.K, ayk_sm_count(), turned, &us);
   const long long tiles = (long long)s.m_tiles * s.n_tiles;
