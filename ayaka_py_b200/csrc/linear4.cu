@@ -629,7 +629,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       for (int first = 0; first < num_kb && ok; first += 4, ++quad) {
         const int q = quad % MANY_QUADS;
         const uint32_t from = come + q * quad_bytes + lane * 16;
-        ok = mbar_wait(come_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 115);
+        ok = mbar_wait_short(come_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 115);
         if (!ok) break;
         uint32_t r[4][4];                    // rows lane, lane + 32, ...: 16 bytes are a row's four column blocks
 #pragma unroll
@@ -637,7 +637,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (first + k >= num_kb || !ok) continue;
-          ok = mbar_wait(bar + to_empty, parity, args.error, 118);
+          ok = mbar_wait_short(bar + to_empty, parity, args.error, 118);
           if (!ok) continue;
           tc_fence_after();
           tmem_st4(columns, r[0][k], r[1][k], r[2][k], r[3][k]);
@@ -683,7 +683,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       int it = 0;
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
         const int buffer = it & 1, t = tile % shape.m_tiles * TILE_T + quarter * 32 + lane, n0 = tile / shape.m_tiles * BN;
-        ok = mbar_wait(sums_full(buffer), (uint32_t)(it >> 1) & 1u, args.error, 117);
+        ok = mbar_wait_short(sums_full(buffer), (uint32_t)(it >> 1) & 1u, args.error, 117);
         if (!ok) break;
         tc_fence_after();
         const uint32_t sums = tmem + ((uint32_t)(quarter * 32) << 16) + buffer * MATRICES * BN;
