@@ -955,6 +955,8 @@ AYK_EXPORT void ayk_linear4_clear_error() { if (g_error_host) *g_error_host = 0;
 // What a product of these sizes runs as: rows of a tile (16, 32 or 64: the few-row kernel, with `parts` CTAs along K to a tile; 128:
 // the many-row kernel, with tiles `parts` features wide).  Host arithmetic.
 AYK_EXPORT int ayk_linear4_plan(int T, int N, int K, int gated, int sms, int* parts) {
+  AYK_REQUIRE(T >= 1 && N >= 1 && K >= MX_BLOCK && K % MX_BLOCK == 0 && sms >= 1 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256,
+              "ayk_linear4_plan: no product of %d rows of %d columns and %d features on %d SMs", T, K, N, sms);
   double us;
   if (!(gated ? takes_few<true>(T, N, K, sms) : takes_few<false>(T, N, K, sms))) {
     *parts = gated ? many_shape<true>(T, N, K, sms, 0, &us).BN : many_shape<false>(T, N, K, sms, N % 16 != 0, &us).BN;

@@ -1880,6 +1880,8 @@ def linear4_plan(T: int, N: int, K: int, gated: bool = False, sms: int = 148) ->
     features wide.  Host arithmetic from the kernels' fitted times: works without a GPU."""
     parts = ctypes.c_int(0)
     rows = library().ayk_linear4_plan(ctypes.c_int(T), ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(1 if gated else 0), ctypes.c_int(sms), ctypes.byref(parts))
+    if rows < 0:
+        _check(rows)
     return rows, parts.value
 
 

@@ -159,6 +159,11 @@ def test_choice_of_a_products_kernel():
     assert ops.linear4_plan(128, 1600, 6400)[0] == 64 and ops.linear4_plan(1024, 1600, 6400)[0] == 128          # 7.4 / 16.6, 29.7 / 18.4 us
     assert ops.linear4_plan(128, 16384, 4096)[0] == 128 and ops.linear4_plan(128, 4096, 16384)[0] == 64          # 21.9 / 13.6, 19.6 / 38.5
     assert ops.linear4_plan(4096, 16384, 4096) == (128, 224) and ops.linear4_plan(4096, 16384, 4096, True) == (128, 96)
+    for bad in ((0, 32, 32), (1, 0, 32), (1, 32, 40), (1, 32, 32, False, 0)):
+        with pytest.raises(ops.KernelError):
+            ops.linear4_plan(*bad)
+    for sms in (1, 7, 20, 132):                                                            # parts of a GPU, other GPUs
+        assert ops.linear4_plan(3, 4096, 4096, False, sms)[0] == 16 and ops.linear4_plan(3000, 4096, 4096, True, sms)[0] in (64, 128)
     widths = {ops.linear4_plan(T, N, K)[1] for T in (100, 300, 1000, 3000) for N in (64, 500, 1600, 4096, 9000) for K in (256, 2048)
               if ops.linear4_plan(T, N, K)[0] == 128}
     assert widths == {32, 64, 96, 128, 192, 224}                                                                # every width has its products
