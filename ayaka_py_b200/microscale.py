@@ -28,8 +28,8 @@ def scale_columns(width: int) -> int:
 
 class Rows8:
     """``codes`` [T, K] float8_e4m3fn and ``scales`` [T, K / 32] float8_e8m0fnu: row t is codes[t, k] * scales[t, k // 32].
-    Tensors that do not lie as the kernels read them (rows of codes and of scales from 16-byte
-    boundaries, columns side by side) are copied into such.  ``apart``: bytes from a row of codes, and of scales, to the next."""
+    Tensors that do not lie as the kernels read them (rows of codes and of scales from 16-byte boundaries, columns side by side) are
+    copied into such.  ``apart``: bytes from a row of codes, and of scales, to the next."""
 
     __slots__ = ("codes", "scales", "apart")
 
