@@ -878,7 +878,7 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
   using L = Few<BT, GATED>;
   constexpr int MOST = MOST_SPLITS<BT, GATED>;
   static_assert(L::smem(MOST) <= 232448 && L::smem(1) <= 232448, "shared memory");
-  static_assert(L::USED <= 512 && 8 * (2 * L::STAGES + 2 * MANY_QUADS + 2) <= 256 && L::AT_BARS % 16 == 0, "layout");
+  static_assert(L::USED <= 512 && 8 * (2 * L::STAGES + 2 * QUADS + 2) <= 256 && L::AT_BARS % 16 == 0, "layout");
   const int tiles_n = (args.N + TILE_N - 1) / TILE_N, tiles_t = (args.T + BT - 1) / BT;
   AYK_REQUIRE(tiles_t <= 65535, "%s: too many rows (%d)", name, args.T);
   const int splits = few_splits<BT, GATED>(args.T, args.N, args.K, ayk_sm_count());
@@ -919,7 +919,7 @@ int launch_many(const void* codes0, const void* codes1, const void* a, long long
   AYK_REQUIRE(tiles <= 0x7fffffff - 65536, "%s: too many rows (%d) and columns (%d)", name, args.T, args.N);
   CUtensorMap w0, w1, rows, row_scales;
   const int padded = args.n_blocks * TILE_N;
-  if (encode_weight(&w0, codes0, padded, args.K, s.BN) != 0 || encode_weight(&w1, codes1, padded, args.K, s.BN) != 0 ||
+  if (encode_weight(&w0, codes0, padded, args.K, s.BN) != 0 || (GATED && encode_weight(&w1, codes1, padded, args.K, s.BN) != 0) ||
       encode_rows(&rows, a, args.T, args.K, a_stride, TILE_T) != 0 || encode_scales(&row_scales, args.a_scales, args.T, args.K, args.a_scale_stride) != 0)
     return -1;
   static AykPerDevice configured;
@@ -933,8 +933,8 @@ int launch_many(const void* codes0, const void* codes1, const void* a, long long
     }
   }
   const int sms = ayk_sm_count();
-  ayk_launch(linear4_many_kernel<GATED>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(MANY_THREADS),
-             (size_t)s.smem, stream, w0, w1, rows, row_scales, args, s);
+  ayk_launch(linear4_many_kernel<GATED>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(MANY_THREADS), (size_t)s.smem, stream, w0, GATED ? w1 : w0, rows,
+             row_scales, args, s);
   return ayk_check_launch(name);
 }
 

@@ -1,8 +1,6 @@
 // Blocks of 32 numbers that share a power of two: rows as e4m3, weights as e2m1, scales as e8m0 (the biased exponent; 255: NaN).
 #pragma once
 
-#include <cuda_fp8.h>
-
 #include "common.cuh"
 
 constexpr int MX_BLOCK = 32;
@@ -18,16 +16,12 @@ __device__ __forceinline__ uint32_t mx_scale_code(uint32_t largest_bits) {
 // 2^-e for a scale's code: the factor that takes numbers to their codes.  (254 - code: the factor's biased exponent; 127 of 2^-127
 // is a plain number, and the largest code that mx_scale_code gives, 247, leaves 7.)
 __device__ __forceinline__ float mx_inverse(uint32_t code) { return __uint_as_float(code == 255u ? 0x7fffffffu : (254u - code) << 23); }
-__device__ __forceinline__ float mx_scale(uint32_t code) { return __uint_as_float(code == 255u ? 0x7fffffffu : code == 0u ? 0x00400000u : code << 23); }
 
 // Two numbers to e4m3, rounded to the nearest (ties to even); the first in the low byte.  A NaN stays one.
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
-}
-__device__ __forceinline__ float e4m3_float(uint32_t byte) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
 }
 // The largest magnitude's bits are compared as whole numbers, so that a NaN is the largest of all.
 __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
