@@ -72,7 +72,8 @@ class Matrix4:
     behind the other, in each the rows (rounded up to whole 128) as 64 bytes (two codes to a byte, the even column in the low
     half); and for every column block and 128 rows the 128 x 4 scales as the tensor cores take them (row r, block b at byte
     16 (r % 32) + 4 (r // 32) + b).  What the last blocks have too much is zeros.  Made by ``Matrix4.from_codes`` or ``matrix4``
-    and complete in memory by then: the kernels may read it ahead of earlier work in their stream, so it is not written to again."""
+    and complete in memory by then (the stream is waited for, so not while one is captured): the kernels may read it ahead of
+    earlier work in their stream, so it is not written to again."""
 
     __slots__ = ("codes", "scales", "shape")
 
@@ -101,13 +102,17 @@ class Matrix4:
         if bool((scales == 255).any()):
             raise FormatError("a scale of the weight is NaN")
         nt, kt = -(-N // TILE), -(-K // TILE)
-        c = torch.zeros((nt * TILE, kt * TILE // 2), dtype=torch.uint8, device=codes.device)
-        c[:N, :K // 2] = codes
-        s = torch.zeros((nt * TILE, kt * TILE // BLOCK), dtype=torch.uint8, device=codes.device)
-        s[:N, :K // BLOCK] = scales
-        c = c.view(nt * TILE, kt, TILE // 2).transpose(0, 1).clone(memory_format=torch.contiguous_format)
-        s = s.view(nt, 4, 32, kt, 4).permute(3, 0, 2, 1, 4).clone(memory_format=torch.contiguous_format).view(kt, nt, TILE * TILE // BLOCK)
-        return cls(c, s, (N, K))
+
+        def whole(t: torch.Tensor, columns: int) -> torch.Tensor:
+            if t.shape == (nt * TILE, columns):
+                return t.contiguous()
+            out = torch.zeros((nt * TILE, columns), dtype=torch.uint8, device=t.device)
+            out[:N, :t.shape[1]] = t
+            return out
+
+        c = whole(codes, kt * TILE // 2).view(nt * TILE, kt, TILE // 2).transpose(0, 1)
+        s = whole(scales, kt * TILE // BLOCK).view(nt, 4, 32, kt, 4).permute(3, 0, 2, 1, 4)
+        return cls(c.clone(memory_format=torch.contiguous_format), s.clone(memory_format=torch.contiguous_format).view(kt, nt, TILE * TILE // BLOCK), (N, K))
 
     def row_major(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(codes, scales as uint8), as ``from_codes`` takes them."""
