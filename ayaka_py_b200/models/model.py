@@ -142,14 +142,14 @@ class Model:
         return seen
 
     def weight_bytes(self) -> int:
-        """Bytes of every distinct bound tensor (a tied table counts once)."""
+        """Bytes of every distinct bound tensor (a tied table counts once), and of what parts keep in their place."""
         seen, total = set(), 0
         for row in self._rows:
             t = getattr(row.part, row.name.replace(".", "_"), None)
             if t is not None and t.data_ptr() not in seen:
                 seen.add(t.data_ptr())
                 total += t.numel() * t.element_size()
-        return total
+        return total + sum(t.numel() * t.element_size() for part in self.parts() for t in part.laid_out())
 
     # ------------------------------------------------------------------ run --
     def forward(self, ctx) -> torch.Tensor:

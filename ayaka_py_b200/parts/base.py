@@ -135,6 +135,10 @@ class Part:
         for name, tensor in tensors.items():
             setattr(self, name.replace(".", "_"), tensor)
 
+    def laid_out(self) -> list[torch.Tensor]:
+        """Tensors that the part keeps in the place of bound ones that it let go of."""
+        return []
+
     def cache_need(self):
         """``KVNeed``, ``StateNeed`` or None."""
         return None

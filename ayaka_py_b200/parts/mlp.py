@@ -50,6 +50,9 @@ class MLP(FeedForward):
             self.up4, self.down4 = matrix4(self.up_weight), matrix4(self.down_weight)
             self.up_weight = self.down_weight = None
 
+    def laid_out(self):
+        return [t for m in (self.up4, self.down4) if m is not None for t in (m.codes, m.scales)]
+
     def forward(self, h, residual, ctx):
         if self.weight_bits == 4:
             u = ops.linear4(ops.rows8(h), self.up4, self.up_bias, self.activation, out_dtype=self.dtype)
@@ -121,6 +124,9 @@ class GatedMLP(FeedForward):
             return
         self.stack = StackedInput(self.width, [[self.gate_weight, self.up_weight]])
         self.gate_weight, self.up_weight = self.stack.views[:2]
+
+    def laid_out(self):
+        return [t for m in self.matrices or () for t in (m.codes, m.scales)]
 
     @property
     def in_weight(self):

@@ -67,7 +67,10 @@ def test_logits_of_prompts_and_single_tokens(dtype):
     steps = [[("a", rs.randint(0, 211, 130).tolist()), ("b", rs.randint(0, 211, 21).tolist())]]
     steps += [[("a", [int(rs.randint(211))]), ("b", [int(rs.randint(211))])] for _ in range(3)]
     steps += [[("a", [7]), ("c", rs.randint(0, 211, 70).tolist())]]
-    got, want = logits_of(model_of(4, dtype), steps), logits_of(model_of(16, torch.float32, rounded=True), steps)
+    small, large = model_of(4, dtype), model_of(16, torch.float32, rounded=True)
+    matrices = 2 * 2 * 128 * 288                              # numbers of the feed-forwards' weights, 4 bytes each in the one model
+    assert small.weight_bytes() < large.weight_bytes() - 4 * matrices + matrices
+    got, want = logits_of(small, steps), logits_of(large, steps)
     assert ops.tc_error() == 0
     for g, w in zip(got, want):
         assert float((g - w).norm() / w.norm()) < (0.07 if dtype == torch.float32 else 0.09)

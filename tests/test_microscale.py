@@ -137,6 +137,15 @@ def test_a_part_binds_its_4_bit_weights():
     w = {name: torch.randn(decl.shape, generator=torch.Generator().manual_seed(1)) for name, decl in part.tensors().items()}
     part.bind(w)
     assert torch.equal(part.up4.decoded(), matrix4(w["up_weight"]).decoded()) and part.down4.shape == (64, 96) and part.up_weight is None
+    assert sum(t.numel() for t in part.laid_out()) == 2 * (128 * 64 + 512)                # one tile each
+    gated = make_part(PartSpec("gated_mlp", {"width": 64, "inner": 96, "activation": "silu", "weight_bits": 4}), torch.float32, "cpu")
+    assert gated.laid_out() == []
+    gated.bind({name: torch.randn(decl.shape, generator=torch.Generator().manual_seed(2)) for name, decl in gated.tensors().items()})
+    assert sum(t.numel() for t in gated.laid_out()) == 3 * (128 * 64 + 512) and gated.join_input(torch.zeros(8, 64), None) is None
+    import copy
+    import pickle
+    for again in (copy.deepcopy(gated), pickle.loads(pickle.dumps(gated))):
+        assert torch.equal(again.matrices[1].decoded(), gated.matrices[1].decoded()) and again.matrices[1].shape == (96, 64)
     with pytest.raises(NotLowered):
         part.lower(None, 0, 0)
 
