@@ -51,6 +51,19 @@ __device__ __forceinline__ uint32_t row_scales(const Args& a, int t, int kb) {
   return word;
 }
 
+// The activations of the tensor-core epilogues, of which the squared ReLU's maximum would take a NaN to 0: here a row that is no number
+// stays so under every one (max.NaN is one instruction as well).
+template <int ACT>
+__device__ __forceinline__ float activated(float x, int act) {
+  if constexpr (ACT == AYK_ACT_RELU2) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+    return r * r;
+  } else {
+    return apply_activation_tc<ACT>(x, act);
+  }
+}
+
 // One feature n (a lane's) of CNT rows from t on.  Linear: bias, activation, residual (every load before the first store: the
 // residual may be C), rounding.  Gated: the warp's 32 features are a block, whose largest magnitude makes the scale.
 // `inside`: n is a feature (of a gated product all 32 or none).
@@ -59,7 +72,7 @@ __device__ __forceinline__ void finish_rows(const Args& a, int t, int n, bool in
   if constexpr (GATED) {
 #pragma unroll
     for (int j = 0; j < CNT; ++j) {
-      const float y = apply_activation_tc<ACT>(v[j], a.act) * u[j];
+      const float y = activated<ACT>(v[j], a.act) * u[j];
       const uint32_t code = mx_scale_code(__reduce_max_sync(0xffffffffu, magnitude_bits(y)));
       if (inside && t + j < a.T) {
         ((uint8_t*)a.C)[(size_t)(t + j) * a.N + n] = (uint8_t)e4m3_pair(y * mx_inverse(code), 0.f);
@@ -74,7 +87,7 @@ __device__ __forceinline__ void finish_rows(const Args& a, int t, int n, bool in
 #pragma unroll
     for (int j = 0; j < CNT; ++j) {
       if (t + j < a.T) {
-        const float y = apply_activation_tc<ACT>(v[j] + b, a.act) + r[j];
+        const float y = activated<ACT>(v[j] + b, a.act) + r[j];
         const size_t at = (size_t)(t + j) * a.N + n;
         if (a.out_bf16) ((__nv_bfloat16*)a.C)[at] = __float2bfloat16_rn(y);
         else ((float*)a.C)[at] = y;
@@ -409,7 +422,7 @@ __device__ __forceinline__ void finish_features(const Args& a, int t, int n, con
     v[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + b.z; v[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + b.w;
   }
 #pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = apply_activation_tc<ACT>(v[j], a.act);
+  for (int j = 0; j < 16; ++j) v[j] = activated<ACT>(v[j], a.act);
   if (a.residual) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] += res[j];
@@ -462,7 +475,7 @@ __device__ __forceinline__ void finish_turned(const Args& a, uint32_t sums, floa
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float y = apply_activation_tc<ACT>(mine[(first + i) * TURNED_ROW + lane] + b, a.act);
+          float y = activated<ACT>(mine[(first + i) * TURNED_ROW + lane] + b, a.act);
           if (a.residual) y += res[i];
           if (first + i < rows) *out = from_float<O>(y);
           out += a.N;
@@ -481,7 +494,7 @@ __device__ __forceinline__ void finish_block(const Args& a, int t, int n, const 
   uint32_t largest = 0u;
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
-    v[j] = apply_activation_tc<ACT>(__uint_as_float(g[j]), a.act) * __uint_as_float(u[j]);
+    v[j] = activated<ACT>(__uint_as_float(g[j]), a.act) * __uint_as_float(u[j]);
     largest = max(largest, magnitude_bits(v[j]));
   }
   const uint32_t code = mx_scale_code(largest);

@@ -1842,8 +1842,8 @@ def rmsnorm_rows8(x: torch.Tensor, weight: torch.Tensor, eps: float, y: torch.Te
 
 def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: str = "none", residual: torch.Tensor | None = None,
             out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
-    """act(a @ w^T + bias) (+ residual): rows in 8 bits times a weight in 4, products exact, sums, activation (as ``linear``) and
-    residual (float32; it may be ``out``) in 32-bit."""
+    """act(a @ w^T + bias) (+ residual): rows in 8 bits times a weight in 4, products exact, sums, activation (as ``linear``, but a
+    NaN stays one under every activation) and residual (float32; it may be ``out``) in 32-bit."""
     lib = _ready()
     codes = a.codes
     (T, K), (N, width), device = codes.shape, w.shape, _current_device()
