@@ -7,7 +7,8 @@
 // Weights lie in column blocks of 128 (64 bytes of codes a row), their scales beside them as the tensor cores take them.  The
 // copy engine spreads sixteen codes over sixteen bytes on their way into shared memory.
 //
-// Every wait is bounded; one that runs out records a code (101 ... 118) in an error word and the CTA winds down.
+// Every wait is bounded; one that runs out records a code (101 ... 119) in an error word and the CTA winds down: whoever gave up, its copies
+// in flight and its MMAs are waited for before it leaves.
 #include <cuda.h>
 
 #include <mutex>
@@ -38,6 +39,33 @@ struct Args {
   int n_blocks;                  // the weight's rows in whole 128
   int act, out_bf16;
 };
+
+// What has to be known to wind a CTA down where a warp has given up, in shared memory behind the barriers.
+struct Ends {
+  uint32_t tmem;                 // the address of tensor memory
+  int issued;                    // stages whose operands are copied
+  int gave_up;
+  int quads, tiles;              // many rows: quads of scales that are copied, tiles whose last product is committed
+};
+
+// A wait for other warps of the CTA, bounded.  (That it gives up at once, to test what comes after, is a constant of a build of its own: a
+// flag in the arguments cost 2 to 9 % of a launch, a vote of a warp's lanes up to 6.  Lanes poll side by side, and give up so.)
+__device__ __forceinline__ bool hand_over(uint32_t bar, uint32_t parity, int* error, int code) {
+#ifdef AYK_IMPATIENT
+  if (mbar_test(bar, parity)) return true;
+  atomicExch(error, code);
+  return false;
+#else
+  return mbar_wait_short(bar, parity, error, code);
+#endif
+}
+__device__ __forceinline__ bool hand_over_warp(uint32_t bar, uint32_t parity, int* error, int code) {
+#ifdef AYK_IMPATIENT
+  return __all_sync(0xffffffffu, hand_over(bar, parity, error, code));
+#else
+  return hand_over(bar, parity, error, code);
+#endif
+}
 
 // The scales of row t for column block kb, the first block in the low byte; zeros (2^-127) beyond the matrix.
 __device__ __forceinline__ uint32_t row_scales(const Args& a, int t, int kb) {
@@ -157,6 +185,7 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
   auto scales_full = [&](int q) { return bars + 8u * (2 * STAGES + q); };
   auto scales_empty = [&](int q) { return bars + 8u * (2 * STAGES + QUADS + q); };
   const uint32_t done_bar = bars + 8u * (2 * STAGES + 2 * QUADS), tmem_slot = done_bar + 8u;
+  volatile Ends* ends = (volatile Ends*)(smem_raw + (tmem_slot - raw));
 
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * TILE_N, t0 = blockIdx.y * BT;
@@ -177,6 +206,7 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
       mbar_init(scales_empty(q), 1);
     }
     mbar_init(done_bar, 1);
+    ends->gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -216,7 +246,7 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
       int issued = pre, s = 0;
       uint32_t parity = 0;
       for (int i = pre; i < num_kb; ++i) {
-        ok = mbar_wait_short(empty_bar(s), parity, args.error, 101);
+        ok = hand_over(empty_bar(s), parity, args.error, 101);
         if (!ok) break;
         mbar_expect_tx(full_bar(s), L::TX);
         load_weights(i, s);
@@ -224,9 +254,8 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
         issued = i + 1;
         if (++s == STAGES) { s = 0; parity ^= 1u; }
       }
-      if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued
-        for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(full_bar(i % STAGES), (uint32_t)(i / STAGES) & 1u, args.error, 102);
-      }
+      ends->issued = issued;
+      if (!ok) ends->gave_up = 1;
     }
     __syncwarp();
     cluster_wait();
@@ -236,8 +265,8 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
       uint32_t bar = full_bar(0), at = 0, scales_at = 0, columns = tmem + L::ACCUMULATORS, parity = 0;      // this stage's: barrier, 16-byte units from the first on, scales
       uint32_t q = 0, quad_parity = 0;
       for (int i = 0; i < num_kb; ++i) {
-        if ((i & 3) == 0) ok = mbar_wait_short(scales_full(q), quad_parity, args.error, 103);
-        ok = ok && mbar_wait_short(bar, parity, args.error, 104);
+        if ((i & 3) == 0) ok = hand_over(scales_full(q), quad_parity, args.error, 103);
+        ok = ok && hand_over(bar, parity, args.error, 104);
         if (!ok) break;
         tc_fence_after();
         // A stage's scales have columns of their own: by the time the stage comes round again the MMAs that read them are done.
@@ -264,6 +293,7 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
         }
       }
       umma_commit(done_bar);     // arrives when every MMA issued so far is done
+      if (!ok) ends->gave_up = 1;
     }
     __syncwarp();
     cluster_wait();
@@ -279,7 +309,7 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
           const int i = quad * 4 + k, r = 32 * j + lane;
           words[j][k] = i < num_kb && r < BT ? row_scales(args, t0 + r, kb0 + i) : 0u;
         }
-      if (quad >= QUADS && !mbar_wait(scales_empty(w), ((uint32_t)(quad / QUADS) & 1u) ^ 1u, args.error, 105)) break;
+      if (quad >= QUADS && !hand_over_warp(scales_empty(w), ((uint32_t)(quad / QUADS) & 1u) ^ 1u, args.error, 105)) break;
 #pragma unroll
       for (int j = 0; j < (BT + 31) / 32; ++j)
 #pragma unroll
@@ -361,6 +391,9 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
   tc_fence_before();
   __syncthreads();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM) : "memory");
+  if (threadIdx.x == 0 && ends->gave_up) {       // each stage's last copies may not have been waited for (they are, where the MMAs ran)
+    for (int i = max(0, ends->issued - STAGES); i < ends->issued; ++i) mbar_wait(full_bar(i % STAGES), (uint32_t)(i / STAGES) & 1u, args.error, 102);
+  }
 }
 
 // --------------------------------------------------------------- many rows --
@@ -385,6 +418,8 @@ constexpr int ROWS_BYTES = TILE_T * BLOCK_K;
 constexpr int MANY_MOST_STAGES = 8;
 constexpr int MANY_QUADS = 2;                   // places of the ring of scales as they come
 constexpr int MANY_MOST_BLOCKS = 3;             // of 128 features' scales that a tile of 224 touches
+constexpr int MANY_BARS_BYTES = 288;            // barriers (three to a stage) and what lies behind them
+static_assert(8 * (3 * MANY_MOST_STAGES + 4 + 2 * MANY_QUADS) + sizeof(Ends) <= MANY_BARS_BYTES && MANY_BARS_BYTES % 16 == 0, "barriers");
 
 struct ManyShape {
   int BN, stages, m_tiles, n_tiles;
@@ -510,6 +545,13 @@ __device__ __forceinline__ void finish_block(const Args& a, int t, int n, const 
 __device__ __forceinline__ void lds_v4(uint32_t at, uint32_t* w) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
 }
+// Where a warp gave up: the last tile's MMAs, each stage's last copies and the scales' last ones.  (Not inline: instructions that no launch runs
+// stood in the way of those behind them.)
+__device__ __noinline__ void wait_for_the_last(uint32_t sums, uint32_t parity, uint32_t full, int issued, int stages, uint32_t come, int quads, int* error) {
+  mbar_wait(sums, parity, error, 112);
+  for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(full + 8u * (i % stages), (uint32_t)(i / stages) & 1u, error, 112);
+  for (int i = max(0, quads - MANY_QUADS); i < quads; ++i) mbar_wait(come + 8u * (i % MANY_QUADS), (uint32_t)(i / MANY_QUADS) & 1u, error, 112);
+}
 template <bool GATED>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
 linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1, const __grid_constant__ CUtensorMap map_a,
@@ -526,7 +568,9 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
   auto sums_empty = [&](int b) { return bars + 8u * (2 * MANY_MOST_STAGES + 2 + b); };
   auto come_full = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 4 + q); };
   auto come_empty = [&](int q) { return bars + 8u * (2 * MANY_MOST_STAGES + 4 + MANY_QUADS + q); };
-  const uint32_t tmem_slot = bars + 8u * (2 * MANY_MOST_STAGES + 4 + 2 * MANY_QUADS);
+  auto scaled_bar = [&](int s) { return bars + 8u * (2 * MANY_MOST_STAGES + 4 + 2 * MANY_QUADS + s); };
+  const uint32_t tmem_slot = scaled_bar(MANY_MOST_STAGES);
+  volatile Ends* ends = (volatile Ends*)(smem_raw + (tmem_slot - raw));
 
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int num_kb = (args.K + BLOCK_K - 1) / BLOCK_K;
@@ -537,7 +581,8 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
     if (GATED) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w1) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
     for (int s = 0; s < stages; ++s) {
-      mbar_init(full_bar(s), 1 + 4);         // the operands' copies and the four warps that bring the scales
+      mbar_init(full_bar(s), 1);             // the operands' copies alone, so that they can be waited for whatever became of the scales
+      mbar_init(scaled_bar(s), 4);           // the four warps that bring the scales
       mbar_init(empty_bar(s), 1);
     }
     for (int q = 0; q < MANY_QUADS; ++q) {
@@ -548,6 +593,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       mbar_init(sums_full(b), 1);
       mbar_init(sums_empty(b), 8);
     }
+    ends->gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -572,7 +618,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
         const int t0 = tile % shape.m_tiles * TILE_T, n0 = tile / shape.m_tiles * BN;
         for (int kb = 0; kb < num_kb; ++kb) {
-          ok = mbar_wait_short(bar + to_empty, parity, args.error, 111);
+          ok = hand_over(bar + to_empty, parity, args.error, 111);
           if (!ok) break;
           mbar_expect_tx(bar, tx);
           tma_load_2d(at, &map_a, kb * BLOCK_K, t0, bar);
@@ -584,23 +630,22 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           if (bar == bars_end) { bar = full_bar(0); at = tiles; parity ^= 1u; }
         }
       }
-      if (!ok) {                 // nobody may be consuming any more: wait for the copies already issued (the scales of each come before long)
-        for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(full_bar(i % stages), (uint32_t)(i / stages) & 1u, args.error, 112);
-      }
+      ends->issued = issued;
+      if (!ok) ends->gave_up = 1;
     }
     __syncwarp();
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = make_idesc_mx(TILE_T, MATRICES * BN, MX_E4M3, MX_E2M1);
-      const uint32_t bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0), all_sums = 2 * MATRICES * BN;
+      const uint32_t bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0), to_scaled = scaled_bar(0) - full_bar(0), all_sums = 2 * MATRICES * BN;
       const uint64_t rows0 = make_desc(tiles), weights0 = make_desc(tiles + ROWS_BYTES);
       uint32_t bar = full_bar(0), at = 0, parity = 0, columns = tmem + all_sums;      // this stage's: barrier, 16-byte units from the first on, scales
       int it = 0;
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
         const uint32_t buffer = it & 1, sums = tmem + buffer * MATRICES * BN;
-        if (it >= 2) ok = mbar_wait_short(sums_empty(buffer), ((uint32_t)(it >> 1) & 1u) ^ 1u, args.error, 113);
+        if (it >= 2) ok = hand_over(sums_empty(buffer), ((uint32_t)(it >> 1) & 1u) ^ 1u, args.error, 113);
         for (int kb = 0; kb < num_kb && ok; ++kb) {
-          ok = mbar_wait_short(bar, parity, args.error, 114);
+          ok = hand_over(bar + to_scaled, parity, args.error, 119) && hand_over(bar, parity, args.error, 114);
           if (!ok) break;
           tc_fence_after();
           const uint64_t rows = rows0 + at, weights = weights0 + at;
@@ -615,6 +660,8 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         }
         umma_commit(sums_full(buffer));
       }
+      ends->tiles = it;
+      if (!ok) ends->gave_up = 1;
     }
     __syncwarp();
   } else if (warp == 14) {
@@ -626,7 +673,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         const int blocks = min((n0 % TILE_N + BN + TILE_N - 1) / TILE_N, args.n_blocks - block0);
         for (int first = 0; first < num_kb; first += 4, ++quads) {
           const int q = quads % MANY_QUADS, kbs = min(4, num_kb - first);
-          if (quads >= MANY_QUADS) ok = mbar_wait_short(come_empty(q), ((uint32_t)(quads / MANY_QUADS) & 1u) ^ 1u, args.error, 116);
+          if (quads >= MANY_QUADS) ok = hand_over(come_empty(q), ((uint32_t)(quads / MANY_QUADS) & 1u) ^ 1u, args.error, 116);
           if (!ok) break;
           mbar_expect_tx(come_full(q), QUAD_BYTES + MATRICES * kbs * blocks * SCALE_BYTES);
           tma_load_2d(come + q * quad_bytes, &map_s, 4 * first, t0, come_full(q));
@@ -636,13 +683,12 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
                         args.w_scales[m] + ((size_t)(first + k) * args.n_blocks + block0) * SCALE_BYTES, blocks * SCALE_BYTES, come_full(q));
         }
       }
-      if (!ok) {
-        for (int i = max(0, quads - MANY_QUADS); i < quads; ++i) mbar_wait(come_full(i % MANY_QUADS), (uint32_t)(i / MANY_QUADS) & 1u, args.error, 112);
-      }
+      ends->quads = quads;
+      if (!ok) ends->gave_up = 1;
     }
     __syncwarp();
   } else if (warp < 4 || warp >= 12) {
-    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 2 * MATRICES * BN, bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0);
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 2 * MATRICES * BN, bars_end = full_bar(stages), to_empty = empty_bar(0) - full_bar(0), to_scaled = scaled_bar(0) - full_bar(0);
     uint32_t bar = full_bar(0), columns = lanes, parity = 1;       // of the stage: the scales' columns are free when the operands' place is
     int quad = 0;
     for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
@@ -650,7 +696,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       for (int first = 0; first < num_kb && ok; first += 4, ++quad) {
         const int q = quad % MANY_QUADS;
         const uint32_t from = come + q * quad_bytes + lane * 16;
-        ok = mbar_wait_short(come_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 115);
+        ok = hand_over_warp(come_full(q), (uint32_t)(quad / MANY_QUADS) & 1u, args.error, 115);
         if (!ok) break;
         uint32_t r[4][4];                    // rows lane, lane + 32, ...: 16 bytes are a row's four column blocks
 #pragma unroll
@@ -658,7 +704,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (first + k >= num_kb || !ok) continue;
-          ok = mbar_wait_short(bar + to_empty, parity, args.error, 118);
+          ok = hand_over_warp(bar + to_empty, parity, args.error, 118);
           if (!ok) continue;
           tc_fence_after();
           tmem_st4(columns, r[0][k], r[1][k], r[2][k], r[3][k]);
@@ -687,7 +733,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar);
+          if (lane == 0) mbar_arrive(bar + to_scaled);
           bar += 8u;
           columns += 4 * groups;
           if (bar == bars_end) { bar = full_bar(0); columns = lanes; parity ^= 1u; }
@@ -696,6 +742,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         if (lane == 0) mbar_arrive(come_empty(q));
       }
     }
+    if (!ok) ends->gave_up = 1;
   } else {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     pdl_wait();
@@ -704,7 +751,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
       int it = 0;
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
         const int buffer = it & 1, t = tile % shape.m_tiles * TILE_T + quarter * 32 + lane, n0 = tile / shape.m_tiles * BN;
-        ok = mbar_wait_short(sums_full(buffer), (uint32_t)(it >> 1) & 1u, args.error, 117);
+        ok = hand_over_warp(sums_full(buffer), (uint32_t)(it >> 1) & 1u, args.error, 117);
         if (!ok) break;
         tc_fence_after();
         const uint32_t sums = tmem + ((uint32_t)(quarter * 32) << 16) + buffer * MATRICES * BN;
@@ -718,7 +765,7 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
             finish_block<ACT>(args, t, n0 + c, g, u);
           }
         } else if (shape.turned) {
-          float* mine = (float*)(smem_raw + (bars + 256 - raw)) + (warp - 4) * 32 * TURNED_ROW;
+          float* mine = (float*)(smem_raw + (bars + MANY_BARS_BYTES - raw)) + (warp - 4) * 32 * TURNED_ROW;
           const int from = half * (BN / 2);
           if (args.out_bf16) finish_turned<ACT, __nv_bfloat16>(args, sums + from, mine, t - lane, n0 + from, BN / 2);
           else finish_turned<ACT, float>(args, sums + from, mine, t - lane, n0 + from, BN / 2);
@@ -736,11 +783,19 @@ linear4_many_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_con
         if (lane == 0) mbar_arrive(sums_empty(buffer));
       }
     });
+    if (!ok) ends->gave_up = 1;
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 1) {
+    if (ends->gave_up) {
+      const int last = ends->tiles - 1;
+      wait_for_the_last(sums_full(last & 1), (uint32_t)(last >> 1) & 1u, full_bar(0), ends->issued, stages, come_full(0), ends->quads, args.error);
+      __syncwarp();
+    }
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
 }
 
 // ------------------------------------------------------------------- host --
@@ -861,7 +916,7 @@ ManyShape many_shape(int T, int N, int K, int sms, int turned, double* us) {
     s.w_touched = ((TILE_N % s.BN == 0 ? 0 : s.BN == 192 ? 64 : 96) + s.BN + TILE_N - 1) / TILE_N;      // a tile starts so far behind a group at most
     const int stage = ROWS_BYTES + MATRICES * s.BN * BLOCK_K;
     s.turned = turned;
-    s.smem = 1024 + MANY_QUADS * (1 + MATRICES * s.w_touched) * QUAD_BYTES + 256 + (turned ? TURNED_BYTES : 0);
+    s.smem = 1024 + MANY_QUADS * (1 + MATRICES * s.w_touched) * QUAD_BYTES + MANY_BARS_BYTES + (turned ? TURNED_BYTES : 0);
     s.stages = (232448 - s.smem) / stage;
     if (s.stages > (512 - 2 * MATRICES * s.BN) / (4 * s.groups)) s.stages = (512 - 2 * MATRICES * s.BN) / (4 * s.groups);      // columns of scales
     if (s.stages > MANY_MOST_STAGES) s.stages = MANY_MOST_STAGES;

@@ -2013,7 +2013,7 @@ MIXED_DECODE_MIN = 1     # single-token requests in a mixed step from which they
 def tc_error() -> int:
     """0, or the code of the bounded wait that ran out in a tensor-core kernel
     (1-4: matrix product, 11-17: attention, 51-58: latent attention, 61-68: per-head products, 80-91: attention of wide heads,
-    101-118: products of 4-bit weights)."""
+    101-119: products of 4-bit weights)."""
     lib = library()
     return (int(lib.ayk_gemm_tc_error()) or int(lib.ayk_attention_tc_error())
             or int(lib.ayk_gemm_tc_prefill_error()) or int(lib.ayk_latent_tc_error()) or int(lib.ayk_head_tc_error())
