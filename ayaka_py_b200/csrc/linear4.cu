@@ -932,11 +932,13 @@ ManyShape many_shape(int T, int N, int K, int sms, int turned, double* us) {
   return best;
 }
 
-// Up to 64 rows every weight byte goes by once in the few-row kernel; above, the quicker one.
+// Up to 64 rows every weight byte goes by once in the few-row kernel; above, the quicker one, where its grid has room.
+constexpr int FEW_MOST_TILES = 65535;      // of rows: a grid's second side
 template <bool GATED>
 bool takes_few(int T, int N, int K, int sms) {
   double many;
   if (T <= 64) return true;
+  if ((T + 63) / 64 > FEW_MOST_TILES) return false;
   many_shape<GATED>(T, N, K, sms, 0, &many);
   return few_us<GATED>(T, N, K, sms) < many;
 }
@@ -948,7 +950,7 @@ int launch_few(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& 
   static_assert(L::smem(MOST) <= 232448 && L::smem(1) <= 232448, "shared memory");
   static_assert(L::USED <= 512 && 8 * (2 * L::STAGES + 2 * QUADS + 2) <= 256 && L::AT_BARS % 16 == 0, "layout");
   const int tiles_n = (args.N + TILE_N - 1) / TILE_N, tiles_t = (args.T + BT - 1) / BT;
-  AYK_REQUIRE(tiles_t <= 65535, "%s: too many rows (%d)", name, args.T);
+  AYK_REQUIRE(tiles_t <= FEW_MOST_TILES, "%s: too many rows (%d)", name, args.T);
   const int splits = few_splits<BT, GATED>(args.T, args.N, args.K, ayk_sm_count());
   static AykPerDevice configured;
   {

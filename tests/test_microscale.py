@@ -178,6 +178,13 @@ def test_choice_of_a_products_kernel():
     assert widths == {32, 64, 96, 128, 192, 224}                                                                # every width has its products
 
 
+@pytest.mark.parametrize("N,K,gated", [(128, 9216, True), (128, 16384, True), (128, 9216, False), (32, 32, False)])
+def test_more_rows_than_a_grid_has_tiles_of_64(N, K, gated):
+    """65,535 tiles of rows at most: more rows go to the kernel whose grid does not grow with them, whichever takes less time."""
+    for T in (65535 * 64 + 1, 65536 * 64, 2 ** 31 - 257):
+        assert ops.linear4_plan(T, N, K, gated)[0] == 128
+
+
 # ------------------------------------------------------- refusals of the calls --
 
 class NoLaunch:
