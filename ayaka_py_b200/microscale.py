@@ -88,6 +88,9 @@ class Matrix4:
             torch.cuda.current_stream(codes.device).synchronize()
         self.codes, self.scales, self.shape = codes, scales, (int(N), int(K))
 
+    def __reduce__(self):
+        return Matrix4, (self.codes, self.scales, self.shape)      # copies and what is read back are waited for as well
+
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Matrix4":
         """From row-major codes, uint8 [N, K / 2] (two to a byte, the even column in the low half), and their scales

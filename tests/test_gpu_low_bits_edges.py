@@ -77,3 +77,24 @@ def test_kernels_whose_waits_run_out_leave_nothing_behind(impatient, monkeypatch
     impatient.ayk_linear4_clear_error()
     assert code in (101, 103, 104, 105, 111, 113, 114, 115, 116, 117, 118, 119)
     assert ops.tc_error() == 0 and all(torch.equal(got, want) for got in later)
+
+
+def test_copies_of_a_matrix_are_complete_when_they_are_handed_out(monkeypatch):
+    import copy
+    import pickle
+    m, waits = random_matrix(300, 256, 1), []
+    here = torch.cuda.current_stream
+
+    class Waited:
+        def __init__(self, device):
+            self.stream = here(device)
+
+        def synchronize(self):
+            waits.append(self.stream)
+            self.stream.synchronize()
+
+    monkeypatch.setattr(torch.cuda, "current_stream", Waited)
+    for again in (copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
+        del waits[:]
+        other = again(m)
+        assert len(waits) == 1 and other.codes.data_ptr() != m.codes.data_ptr() and torch.equal(other.decoded(), m.decoded())

@@ -150,6 +150,24 @@ def test_a_part_binds_its_4_bit_weights():
         part.lower(None, 0, 0)
 
 
+@pytest.mark.parametrize("again", ["copy", "deepcopy", "pickle"])
+def test_copies_of_a_matrix_pass_through_its_constructor(again, monkeypatch):
+    """Which waits until the matrix is complete in memory: the kernels read it ahead of earlier work in their stream."""
+    import copy
+    import pickle
+    made, init = [], Matrix4.__init__
+
+    def counted(self, codes, scales, shape):
+        made.append(shape)
+        init(self, codes, scales, shape)
+
+    monkeypatch.setattr(Matrix4, "__init__", counted)
+    m = matrix4(torch.randn(130, 96, generator=torch.Generator().manual_seed(3)))
+    del made[:]
+    other = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x))}[again](m)
+    assert made == [(130, 96)] and other.shape == m.shape and torch.equal(other.codes, m.codes) and torch.equal(other.scales, m.scales)
+
+
 # --------------------------------------------------------- the kernels' choices --
 
 def test_choice_of_a_products_kernel():
