@@ -27,8 +27,8 @@ def _check_bits(weight_bits: int, activation: str, *widths: int) -> int:
 class MLP(FeedForward):
     KIND = "mlp"
 
-    def __init__(self, width: int, inner: int, activation: str, bias: bool = True, weight_bits: int = 16,
-                 dtype=torch.float32, device="cuda"):
+    def __init__(self, width: int, inner: int, activation: str, bias: bool = True,
+                 dtype=torch.float32, device="cuda", weight_bits: int = 16):
         if activation not in ops.ACTIVATIONS:
             raise ValueError(f"unknown activation {activation!r}; known: {sorted(ops.ACTIVATIONS)}")
         self.width, self.inner, self.activation, self.has_bias = width, inner, activation, bias
@@ -103,7 +103,7 @@ class GatedMLP(FeedForward):
     KIND = "gated_mlp"
 
     def __init__(self, width: int, inner: int, activation: str, limit: float | None = None, slope: float = 1.702, plus: float = 1.0,
-                 weight_bits: int = 16, dtype=torch.float32, device="cuda"):
+                 dtype=torch.float32, device="cuda", weight_bits: int = 16):
         if activation != "limited_glu" and activation not in ops.ACTIVATIONS:
             raise ValueError(f"unknown activation {activation!r}; known: {sorted(ops.ACTIVATIONS)} and 'limited_glu'")
         self.width, self.inner, self.activation, self.dtype = width, inner, activation, dtype

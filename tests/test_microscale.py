@@ -130,6 +130,13 @@ def test_feed_forwards_that_cannot_have_4_bit_weights(kind, params):
         make_part(PartSpec(kind, {"weight_bits": 4, **params}), torch.bfloat16, "cpu")
 
 
+def test_feed_forwards_take_their_arguments_in_the_order_that_they_had():
+    from ayaka_py_b200.parts.mlp import MLP, GatedMLP
+    plain = MLP(64, 96, "gelu_tanh", False, torch.bfloat16, "cpu")
+    gated = GatedMLP(64, 96, "silu", None, 1.702, 1.0, torch.bfloat16, "cpu")
+    assert plain.dtype == gated.dtype == torch.bfloat16 and plain.weight_bits == gated.weight_bits == 16
+
+
 def test_a_part_binds_its_4_bit_weights():
     from ayaka_py_b200.parts import PartSpec, make_part
     from ayaka_py_b200.parts.base import NotLowered
