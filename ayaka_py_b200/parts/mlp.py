@@ -130,7 +130,8 @@ class GatedMLP(FeedForward):
 
     @property
     def in_weight(self):
-        return self.stack.weight
+        """gate | up in one matrix (None where the weights are 4-bit)."""
+        return None if self.weight_bits == 4 else self.stack.weight
 
     def join_input(self, weight, bias):
         if self.weight_bits == 4:

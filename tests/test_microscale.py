@@ -130,6 +130,18 @@ def test_feed_forwards_that_cannot_have_4_bit_weights(kind, params):
         make_part(PartSpec(kind, {"weight_bits": 4, **params}), torch.bfloat16, "cpu")
 
 
+@pytest.mark.parametrize("weight_bits", [16, 4])
+def test_the_joined_matrix_of_a_gated_feed_forward(weight_bits):
+    from ayaka_py_b200.parts import PartSpec, make_part
+    part = make_part(PartSpec("gated_mlp", {"width": 64, "inner": 96, "activation": "silu", "weight_bits": weight_bits}), torch.float32, "cpu")
+    w = {name: torch.randn(decl.shape, generator=torch.Generator().manual_seed(4)) for name, decl in part.tensors().items()}
+    part.bind(w)
+    if weight_bits == 4:
+        assert part.in_weight is None
+    else:
+        assert torch.equal(part.in_weight, torch.cat((w["gate_weight"], w["up_weight"])))
+
+
 def test_feed_forwards_take_their_arguments_in_the_order_that_they_had():
     from ayaka_py_b200.parts.mlp import MLP, GatedMLP
     plain = MLP(64, 96, "gelu_tanh", False, torch.bfloat16, "cpu")
