@@ -1010,7 +1010,7 @@ int launch_many(const void* codes0, const void* codes1, const void* a, long long
 
 int check(const char* name, const void* a, long long a_stride, const void* a_scales, long long a_scale_stride, long long T, int N, int K, int act) {
   AYK_REQUIRE(N > 0 && K > 0 && K % MX_BLOCK == 0, "%s: a product of %d columns over rows of %d (whole blocks of %d)", name, N, K, MX_BLOCK);
-  AYK_REQUIRE(T >= 0 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256, "%s: too many rows (%lld) or columns (%d)", name, T, N);
+  AYK_REQUIRE(T >= 0 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256 && K <= 0x7fffffff - 256, "%s: too many rows (%lld) or columns (%d, %d)", name, T, N, K);
   AYK_REQUIRE(act >= AYK_ACT_NONE && act <= AYK_ACT_SILU, "%s: unknown activation %d", name, act);
   AYK_REQUIRE((uintptr_t)a % 16 == 0 && a_stride % 16 == 0 && a_stride >= K, "%s: rows of codes must lie on 16-byte boundaries", name);
   AYK_REQUIRE((uintptr_t)a_scales % 16 == 0 && a_scale_stride % 16 == 0 && a_scale_stride >= K / MX_BLOCK, "%s: rows of scales must lie on 16-byte boundaries", name);
@@ -1025,7 +1025,7 @@ AYK_EXPORT void ayk_linear4_clear_error() { if (g_error_host) *g_error_host = 0;
 // What a product of these sizes runs as: rows of a tile (16, 32 or 64: the few-row kernel, with `parts` CTAs along K to a tile; 128:
 // the many-row kernel, with tiles `parts` features wide).  Host arithmetic.
 AYK_EXPORT int ayk_linear4_plan(int T, int N, int K, int gated, int sms, int* parts) {
-  AYK_REQUIRE(T >= 1 && N >= 1 && K >= MX_BLOCK && K % MX_BLOCK == 0 && sms >= 1 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256,
+  AYK_REQUIRE(T >= 1 && N >= 1 && K >= MX_BLOCK && K % MX_BLOCK == 0 && sms >= 1 && T <= 0x7fffffff - 256 && N <= 0x7fffffff - 256 && K <= 0x7fffffff - 256,
               "ayk_linear4_plan: no product of %d rows of %d columns and %d features on %d SMs", T, K, N, sms);
   double us;
   if (!(gated ? takes_few<true>(T, N, K, sms) : takes_few<false>(T, N, K, sms))) {

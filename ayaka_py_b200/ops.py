@@ -1879,6 +1879,8 @@ def linear4_plan(T: int, N: int, K: int, gated: bool = False, sms: int = 148) ->
     """How ``linear4`` (``gated``: ``gated_linear4``) runs T rows of K columns times N features on ``sms`` SMs: (rows of a tile, parts).
     16, 32 or 64 rows: the kernel for few rows, with that many CTAs along K to a tile; 128: the one for many, with tiles that many
     features wide.  Host arithmetic from the kernels' fitted times: works without a GPU."""
+    if not all(0 < n < 2 ** 31 for n in (T, N, K, sms)) or (gated and N % BLOCK):
+        raise KernelError(f"linear4_plan: no {'gated ' if gated else ''}product of {T} rows of {K} columns and {N} features on {sms} SMs")
     parts = ctypes.c_int(0)
     rows = library().ayk_linear4_plan(ctypes.c_int(T), ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(1 if gated else 0), ctypes.c_int(sms), ctypes.byref(parts))
     if rows < 0:

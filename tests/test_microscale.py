@@ -215,6 +215,14 @@ def test_choice_of_a_products_kernel():
     assert widths == {32, 64, 96, 128, 192, 224}                                                                # every width has its products
 
 
+@pytest.mark.parametrize("bad", [(2 ** 32 + 5, 64, 64), (5, 2 ** 32 + 64, 64), (5, 64, 2 ** 32 + 64), (2 ** 31 - 200, 64, 64), (5, 64, 64, False, 2 ** 32 + 1),
+                                 (5, 40, 64, True), (-1, 64, 64), (5, 64, 2 ** 31 - 32)])
+def test_no_plan_for_what_is_no_product(bad):
+    """Numbers beyond 32 bits among them, and gated products whose rows are not whole blocks: those the calls refuse as well."""
+    with pytest.raises(ops.KernelError):
+        ops.linear4_plan(*bad)
+
+
 @pytest.mark.parametrize("N,K,gated", [(128, 9216, True), (128, 16384, True), (128, 9216, False), (32, 32, False)])
 def test_more_rows_than_a_grid_has_tiles_of_64(N, K, gated):
     """65,535 tiles of rows at most: more rows go to the kernel whose grid does not grow with them, whichever takes less time."""
