@@ -816,7 +816,11 @@ int setup() {
   cudaError_t err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
   if (err != cudaSuccess || fn == nullptr || q != cudaDriverEntryPointSuccess) return ayk_fail("ayk_linear4: cuTensorMapEncodeTiled is not available from this driver");
   if (!g_error_host) {
+    // the first call may be one that is captured, which bars its thread from allocations unless it says that they may be made
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     err = cudaHostAlloc((void**)&g_error_host, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (err != cudaSuccess) return ayk_fail("ayk_linear4: cudaHostAlloc: %s", cudaGetErrorString(err));
     *g_error_host = 0;
   }

@@ -2,6 +2,8 @@
 
 import ctypes
 import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 
@@ -98,3 +100,34 @@ def test_copies_of_a_matrix_are_complete_when_they_are_handed_out(monkeypatch):
         del waits[:]
         other = again(m)
         assert len(waits) == 1 and other.codes.data_ptr() != m.codes.data_ptr() and torch.equal(other.decoded(), m.decoded())
+
+
+FIRST_CALL = """
+import sys
+import torch
+from ayaka_py_b200 import ops
+from ayaka_py_b200.microscale import Rows8, matrix4
+kind, T = sys.argv[1], int(sys.argv[2])
+x, w = torch.randn(T, 256, device="cuda"), matrix4(torch.randn(128, 256, device="cuda"))
+a = Rows8(torch.randn(T, 256, device="cuda").to(torch.float8_e4m3fn), torch.full((T, 8), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu))
+norm = torch.ones(256, device="cuda")
+def run():
+    if kind == "linear":
+        return ops.linear4(a, w)
+    rows = ops.rows8(x) if kind == "rows" else ops.rmsnorm_rows8(x, norm, 1e-6) if kind == "norm" else ops.gated_linear4(a, w, w)
+    return rows.decoded()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = run()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, run()) and bool(torch.isfinite(y).all())
+"""
+
+
+@pytest.mark.parametrize("kind", ["rows", "norm", "linear", "gated"])
+@pytest.mark.parametrize("T", [3, 300])
+def test_a_process_whose_first_call_is_captured(kind, T):
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL, kind, str(T)], cwd=str(Path(__file__).resolve().parent.parent), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
