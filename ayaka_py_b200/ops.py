@@ -1843,7 +1843,7 @@ def rmsnorm_rows8(x: torch.Tensor, weight: torch.Tensor, eps: float, y: torch.Te
 def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: str = "none", residual: torch.Tensor | None = None,
             out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """act(a @ w^T + bias) (+ residual): rows in 8 bits times a weight in 4, products exact, sums, activation (as ``linear``, but a
-    NaN stays one under every activation) and residual (float32; it may be ``out``) in 32-bit."""
+    NaN stays one under every activation) and residual (float32; it may be ``out``, but not overlap it otherwise) in 32-bit."""
     lib = _ready()
     codes = a.codes
     (T, K), (N, width), device = codes.shape, w.shape, _current_device()
@@ -1863,6 +1863,10 @@ def linear4(a: Rows8, w: Matrix4, bias: torch.Tensor | None = None, activation: 
         residual_at = residual.data_ptr()
     if out is not None and (tuple(out.shape) != (T, N) or out.dtype != out_dtype or not out.is_contiguous()):
         raise KernelError("linear4: out must be a contiguous [T, N] tensor of the output dtype")
+    if residual is not None and out is not None and out is not residual:
+        at, size = out.data_ptr(), out.element_size()
+        if residual_at < at + T * N * size and at < residual_at + T * N * 4 and (at != residual_at or size != 4):
+            raise KernelError("linear4: residual may be out, but not overlap it otherwise")
     if (codes.get_device() != device or w.codes.get_device() != device or (bias is not None and bias.get_device() != device)
             or (residual is not None and residual.get_device() != device) or (out is not None and out.get_device() != device)):
         raise _elsewhere("linear4", device, codes, w.codes, bias, residual, out)

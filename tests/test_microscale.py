@@ -277,3 +277,18 @@ def test_refused_calls(call, words, monkeypatch):
     monkeypatch.setattr(ops, "_current_device", lambda: 0)
     with pytest.raises(ops.KernelError, match=words):
         call()
+
+
+@pytest.mark.parametrize("dtype,out_at,residual_at,refused", [
+    (torch.float32, 0, 0, False), (torch.float32, 0, 4 * 32, False), (torch.float32, 4 * 32, 0, False), (torch.float32, 0, 32, True), (torch.float32, 32, 0, True),
+    (torch.float32, 1, 0, True), (torch.float32, 0, 4 * 32 - 1, True), (torch.bfloat16, 0, 0, True), (torch.bfloat16, 0, 32, True), (torch.bfloat16, 0, 64, False),
+    (torch.bfloat16, 2 * 4 * 32, 0, False), (torch.bfloat16, 2 * 4 * 32 - 2, 0, True)])
+def test_a_residual_that_overlaps_the_result(dtype, out_at, residual_at, refused, monkeypatch):
+    """Four rows of 32, from any number of one store on: the same place or apart (then the call goes on to where the tensors are)."""
+    monkeypatch.setattr(ops, "_ready", lambda: NoLaunch())
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
+    store = torch.zeros(512)
+    out = store.view(dtype)[out_at:out_at + 128].view(4, 32)
+    residual = store[residual_at:residual_at + 128].view(4, 32)
+    with pytest.raises(ops.KernelError, match="overlap" if refused else "current device"):
+        ops.linear4(rows_of(4, 64), matrix4(torch.ones(32, 64)), residual=residual, out_dtype=dtype, out=out)
