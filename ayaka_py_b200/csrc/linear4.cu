@@ -138,8 +138,8 @@ __device__ __forceinline__ void with_activation(int act, Run run) {
 // A CTA takes 128 features as the MMA's M side and BT rows as its N side, so that a handful of rows streams every weight byte
 // once; the CTAs of a cluster along z share the tile, each with a part of its column blocks, and exchange their 32-bit sums
 // through shared memory.  Bound by the weight's bytes where there are enough, else by the way of one launch: 8 x 16384 x 4096
-// (36 MB) 8.5 us with the weight in L2, 9.8 with weights from memory in turn (3.7 TB/s; each further 36 MB 6 us, 6.1 TB/s); 1 x 1600 x
-// 4800 4.1 us, 128 x 128 alone 1.7.  The MMAs (128 x 16 x 32, 40 clocks: 128 rows' 32 bytes leave shared memory at 128 a clock) would
+// (36 MB) 8.4 us with the weight in L2, 9.6 with weights from memory in turn (3.7 TB/s; each further 36 MB 6 us, 6.1 TB/s); 1 x 1600 x
+// 4800 4.1 us, 128 x 128 alone 1.9.  The MMAs (128 x 16 x 32, 40 clocks: 128 rows' 32 bytes leave shared memory at 128 a clock) would
 // take weights at twice the memory's rate.  Tried, 8 x 16384 x 4096 from memory: three or four stages a CTA 10.9, 10.3; one CTA to a
 // multiprocessor, so that the next launch's fits beside it, 11.2.
 //
@@ -400,8 +400,8 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_cons
 // Persistent CTAs over tiles of 128 rows (the MMA's M side, a row to a lane of tensor memory) by BN features (its N side; of a
 // gated product BN of each matrix, one behind the other), two accumulators in tensor memory so that a tile's epilogue runs under the
 // next one's main loop.  An epilogue thread owns a row and stores runs of features.  Bound by the MMAs and what the operands' and
-// results' ways cost beside them: 4096 x 4096 x 16384 207 us (2.65 PFLOP/s) in short runs; without the epilogue 177, without the
-// operands' copies 162, the MMAs alone 146; 250 us in long ones, where the power cap holds the clock at 1.3 to 1.6 GHz.
+// results' ways cost beside them: 4096 x 4096 x 16384 208 us (2.64 PFLOP/s) in short runs; without the epilogue 177, without the
+// operands' copies 162, the MMAs alone 146; 243 us in long ones, where the power cap holds the clock at 1.3 to 1.6 GHz.
 //
 // Scales travel for four column blocks (a quad) at a time, as they lie in memory.  Four warps, one to a quarter of the lanes of
 // tensor memory, put them there: the rows' turned (16 bytes come for each row), the weights' shifted so that a tile's first feature has
@@ -892,10 +892,12 @@ int few_splits(int T, int N, int K, int sms) {
   return best;
 }
 
-// Microseconds of the two kernels, fitted to graphs of 20 launches each on a B200 (N and K from 768 to 16384, 65 to 1024 rows; off by
-// up to 20 %): per wave of CTAs a fixed part and one per column block.  Both sides of the choice, us few / many: 128 x 6400 x 1600 7.4
-// / 16.6, 512 x 6400 x 1600 14.9 / 17.6, 1024 x 6400 x 1600 29.7 / 18.4, 128 x 4096 x 16384 21.9 / 13.6, gated 256 x 4096 x 4096 17.6 /
-// 16.5, gated 128 x 16384 x 4096 28.6 / 48.3.
+// Microseconds of the two kernels, fitted to graphs of 20 launches each on a B200 (N and K from 768 to 16384, 65 to 1024 rows): per wave of
+// CTAs a fixed part and one per column block.  The estimates are 0.78 to 1.21 times what the kernel for few rows takes (0.97 in the median),
+// but 0.88 to 1.53 times what the one for many takes (1.25): they are of a form of it whose scales were copied by tcgen05.cp.  Both sides of
+// the choice as they are now, us few / many: 128 x 6400 x 1600 7.4 / 12.5, 1024 x 6400 x 1600 29.5 / 14.1, 128 x 4096 x 16384 21.9 / 10.6, gated
+// 128 x 16384 x 4096 28.4 / 36.9, each of which goes to the quicker one; but 512 x 6400 x 1600 14.8 / 13.0, gated 256 x 4096 x 4096 17.7 / 12.2
+// (to the quicker one) and gated 384 x 6400 x 1600 23.5 / 16.2: of 112 products 18 go to the slower kernel, which costs 7 to 45 % there.
 template <bool GATED>
 double few_us(int T, int N, int K, int sms) {
   const int splits = few_splits<64, GATED>(T, N, K, sms), blocks = (K + BLOCK_K - 1) / BLOCK_K;
